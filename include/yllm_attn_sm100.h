@@ -494,6 +494,68 @@ int yattn_sess_kv_save(const uint16_t* kv_dev, uint32_t n_blocks, uint32_t kv_di
 int yattn_sess_kv_load(uint16_t* kv_dev, uint32_t n_blocks, uint32_t kv_dim, uint32_t max_seq,
                        const char* path, uint32_t* pos, void* stream, char* err, size_t errlen);
 
+/* ------------------------------------------------ paged KV cache
+ * Requests that grow share one pool of pages instead of one contiguous cache
+ * each.  A page is page_size (16/32/64/128/256) consecutive rows of a K pool
+ * and of a V pool, both fp16 [n_pages*page_size][kv_dim] with the row layout
+ * of the contiguous cache; row index = slot = page*page_size + offset.  Every
+ * layer has its own pair of pools (or its own base in one allocation); block
+ * tables and slots are shared by the layers.  A serving step is one
+ * yattn_page_step, then per layer yattn_rope_store_kv_paged and
+ * yattn_attn_paged; all of them read lengths on the device, so a step can be
+ * captured in a CUDA graph and replayed with other lengths. */
+
+enum { YATTN_ACT_F32 = 0, YATTN_ACT_F16 = 1, YATTN_ACT_BF16 = 2 };   /* activation types */
+
+/* Block tables, slot maps and the page queue of one step, on the device.
+ * Request r holds kv_len[r] cached tokens in the pages tables[r*table_stride
+ * + 0..] (ceil(kv_len/page_size) of them) and gets new_len[r] >= 0 tokens;
+ * new_len[r] = -1 ends it and returns its pages.  ring[n_pages] is the queue
+ * of free pages: state[0] = index of its head, state[1] = pages in it.
+ * Results, all int32:
+ *   cu_new[n_seqs+1]   prefix sums of the new tokens; token cu_new[r]+i is new
+ *                      token i of request r
+ *   slots[max_tokens]  cache row of each token, -1 from cu_new[n_seqs] on
+ *   positions[...]     its position kv_len[r]+i, 0 from cu_new[n_seqs] on
+ *   kv_len_out[n_seqs] lengths after the step (0 for an ended request)
+ *   tables             the new pages' entries (others stay as they are)
+ *   ring               the ended requests' pages behind the tail
+ *   state_out[4]       the queue's {head, count}, verdict, number of tokens
+ * Pages are handed out from the head in request order, then page order.
+ * Verdict 0 = done; else nothing was handed out or returned, kv_len_out =
+ * kv_len, cu_new is all zero and every slot -1 (so the calls that read them do
+ * nothing): > 0 = pages missing, -1 = more than max_tokens tokens, -2 = a
+ * request needs more than max_pages pages, -3 = malformed lengths or queue.
+ * The inputs kv_len, new_len and state stay as they are and must not overlap
+ * the outputs: feed kv_len_out and state_out to the next step (two sets of
+ * buffers in turn).  state_out is 16-byte aligned.  1 to 16384 requests. */
+int yattn_page_step(int32_t* kv_len_out, int32_t* cu_new, int32_t* slots, int32_t* positions,
+                    uint32_t max_tokens, int32_t* state_out, int32_t* tables, uint32_t max_pages,
+                    uint32_t table_stride, int32_t* ring, uint32_t n_pages, const int32_t* state,
+                    const int32_t* kv_len, const int32_t* new_len, uint32_t n_seqs, uint32_t page_size,
+                    void* stream, char* err, size_t errlen);
+
+/* QK-norm (optional), RoPE and the K/V store of n_tokens tokens into pages:
+ * q_out[t] = rotated q[t]; rotated k[t] and v[t] go to pool row slots[t] with
+ * the engine's f32_to_f16.  q, k, v and q_out hold activations of type `act`
+ * (YATTN_ACT_*), heads contiguous, tokens *_stride elements apart (so q, k and
+ * v may be columns of one projection output); q_out may be q itself with the
+ * same stride.  A token with slot < 0 is skipped: its rows are neither read
+ * nor written.  A slot outside the pool's n_rows rows is not stored and sets
+ * device status 602.  Two tokens with one slot: either may remain.
+ * rope_kind, n_rope_dims (kind 2: a multiple of 16) and qk_norm as
+ * yattn_rope_store_kv, but the angle position*theta^(-2j/n) is taken in 64
+ * bits (that call's fp32 angle drifts by half an ulp of itself at far
+ * positions).  head_dim 64/128/256.  q, k, v, q_out and the pools are 16-byte
+ * aligned, strides multiples of 16 bytes, kv_dim a multiple of 8. */
+int yattn_rope_store_kv_paged(void* q_out, uint32_t q_out_stride, const void* q, uint32_t q_stride,
+                              const void* k, uint32_t k_stride, const void* v, uint32_t v_stride, int act,
+                              uint16_t* kpool, uint16_t* vpool, uint64_t n_rows, const int32_t* slots,
+                              const int32_t* positions, uint32_t n_tokens, uint32_t n_heads,
+                              uint32_t n_kv_heads, uint32_t head_dim, uint32_t kv_dim, int rope_kind,
+                              uint32_t n_rope_dims, float theta, const YattnQkNorm* qk_norm, void* stream,
+                              char* err, size_t errlen);
+
 /* ------------------------------------------------ seeded input generator
  * Deterministic on every device and bit-identical to the CPU restatement in
  * the test oracle: splitmix64 (platform.c:411-417) draws, Box-Muller with

@@ -159,6 +159,9 @@ PROTOS = {
     ),
     "yattn_gen_gdn_gates": (C.c_int, [vp, vp, u64, u64, u64, sz, vp, *E]),
     "yattn_gen_gdn_qk": (C.c_int, [vp, u64, u64, sz, u32, u32, C.c_float, vp, *E]),
+    "yattn_page_step": (C.c_int, [vp, vp, vp, vp, u32, vp, vp, u32, u32, vp, u32, vp, vp, vp, u32, u32, vp, *E]),
+    "yattn_rope_store_kv_paged": (C.c_int, [vp, u32, vp, u32, vp, u32, vp, u32, C.c_int, vp, vp, u64, vp, vp, u32, u32,
+                                            u32, u32, u32, C.c_int, u32, C.c_float, vp, vp, *E]),
     "yattn_checksum": (C.c_int, [vp, sz, C.POINTER(u64), vp, *E]),
 }
 

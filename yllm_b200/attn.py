@@ -401,6 +401,109 @@ def gemv_f16(y: torch.Tensor, w: torch.Tensor, x: torch.Tensor, out: int, in_: i
     call("yattn_gemv_f16", y.data_ptr(), w.data_ptr(), x.data_ptr(), out, in_, B, _stream(stream))
 
 
+# ------------------------------------------------------------- paged KV cache
+
+_ACT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # YATTN_ACT_*
+_F16_BITS = (torch.float16, torch.uint16, torch.int16)
+
+
+def _call_on(name: str, t: torch.Tensor, stream, *args) -> None:
+    """call() on t's device: the given stream of it, or its current one."""
+    dev = t.device.index
+    if stream is None:
+        stream = torch.cuda.current_stream(dev)
+    elif stream.device_index != dev:
+        raise ValueError(f"{name}: the stream is on cuda:{stream.device_index}, the tensors on cuda:{dev}")
+    if dev == torch.cuda.current_device():
+        call(name, *args, stream.cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, stream.cuda_stream)
+
+
+def _i32_on(ref: torch.Tensor, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.dtype != torch.int32 or t.device != ref.device or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor on {ref.device}")
+
+
+def _tables(tables: torch.Tensor, ref: torch.Tensor) -> None:
+    if (tables.dtype != torch.int32 or tables.device != ref.device or tables.dim() != 2 or tables.shape[1] == 0
+            or tables.stride(1) != 1 or (tables.shape[0] > 1 and tables.stride(0) < tables.shape[1])):
+        raise ValueError(f"tables must be an int32 [requests, pages] tensor on {ref.device} with contiguous rows")
+
+
+def _table_stride(tables: torch.Tensor) -> int:
+    return tables.stride(0) if tables.shape[0] > 1 else tables.shape[1]
+
+
+def _pools(kpool: torch.Tensor, vpool: torch.Tensor, n_kv_heads: int, head_dim: int) -> None:
+    for name, t in (("kpool", kpool), ("vpool", vpool)):
+        if not t.is_cuda or t.dtype not in _F16_BITS or t.dim() != 3 or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous CUDA fp16 tensor [pages, page_size, kv_dim]")
+    if kpool.shape != vpool.shape or kpool.device != vpool.device:
+        raise ValueError("kpool and vpool must have the same shape and device")
+    if kpool.shape[2] < n_kv_heads * head_dim:
+        raise ValueError("the pools' rows are shorter than n_kv_heads * head_dim")
+
+
+def _tokens(t: torch.Tensor, name: str, like: torch.Tensor, cols: int) -> None:
+    if (t.dim() != 2 or t.dtype != like.dtype or t.device != like.device or t.shape[0] != like.shape[0]
+            or t.shape[1] != cols or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < cols)):
+        raise ValueError(f"{name} must be [{like.shape[0]}, {cols}] {like.dtype} on {like.device}, heads contiguous")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def page_step(kv_len_out: torch.Tensor, cu_new: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor,
+              state_out: torch.Tensor, tables: torch.Tensor, ring: torch.Tensor, state: torch.Tensor,
+              kv_len: torch.Tensor, new_len: torch.Tensor, page_size: int, stream=None) -> None:
+    """One serving step's block tables (tables and the free-page queue ring updated in place), slots and positions
+    of the new tokens (slots.numel() is the token capacity), prefix sums and lengths, from kv_len and new_len (-1:
+    the request ended).  state_out = {head, count, verdict, tokens}; see yattn_page_step for the verdicts."""
+    if not kv_len.is_cuda:
+        raise ValueError("kv_len must be a CUDA tensor")
+    _i32_on(kv_len, kv_len_out=kv_len_out, cu_new=cu_new, slots=slots, positions=positions, state_out=state_out,
+            ring=ring, state=state, kv_len=kv_len, new_len=new_len)
+    _tables(tables, kv_len)
+    n = kv_len.numel()
+    if new_len.numel() != n or kv_len_out.numel() != n or cu_new.numel() != n + 1 or tables.shape[0] != n:
+        raise ValueError("new_len, kv_len_out, cu_new (one more) and tables must have one entry per request of kv_len")
+    if positions.numel() != slots.numel() or state.numel() < 2 or state_out.numel() < 4:
+        raise ValueError("positions must match slots; state holds 2 values or more, state_out 4")
+    _call_on("yattn_page_step", kv_len, stream, kv_len_out.data_ptr(), cu_new.data_ptr(), slots.data_ptr(),
+             positions.data_ptr(), slots.numel(), state_out.data_ptr(), tables.data_ptr(), tables.shape[1],
+             _table_stride(tables), ring.data_ptr(), ring.numel(), state.data_ptr(), kv_len.data_ptr(),
+             new_len.data_ptr(), n, page_size)
+
+
+def rope_store_kv_paged(q_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kpool: torch.Tensor,
+                        vpool: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor, n_heads: int,
+                        n_kv_heads: int, head_dim: int, rope_kind: int, theta: float, n_rope_dims: int = 0, norm=None,
+                        stream=None) -> None:
+    """QK-norm (norm = qk_norm(...)), RoPE and the store of k and v into pages: q, k, v [tokens, heads*head_dim]
+    (fp32, fp16 or bf16, any row stride), slots and positions from page_step; tokens with slot -1 are skipped.
+    q_out may be q."""
+    if not q.is_cuda or q.dtype not in _ACT:
+        raise ValueError("q must be a CUDA tensor of float32, float16 or bfloat16")
+    for name, t, cols in (("q", q, n_heads * head_dim), ("q_out", q_out, n_heads * head_dim),
+                          ("k", k, n_kv_heads * head_dim), ("v", v, n_kv_heads * head_dim)):
+        _tokens(t, name, q, cols)
+    _pools(kpool, vpool, n_kv_heads, head_dim)
+    if kpool.device != q.device:
+        raise ValueError("the pools must be on q's device")
+    _i32_on(q, slots=slots, positions=positions)
+    if slots.numel() != q.shape[0] or positions.numel() != q.shape[0]:
+        raise ValueError("slots and positions must have one entry per row of q")
+    _call_on("yattn_rope_store_kv_paged", q, stream, q_out.data_ptr(), _row_stride(q_out), q.data_ptr(),
+             _row_stride(q), k.data_ptr(), _row_stride(k), v.data_ptr(), _row_stride(v), _ACT[q.dtype],
+             kpool.data_ptr(), vpool.data_ptr(), kpool.shape[0] * kpool.shape[1], slots.data_ptr(),
+             positions.data_ptr(), q.shape[0], n_heads, n_kv_heads, head_dim, kpool.shape[2], rope_kind, n_rope_dims,
+             theta, _norm_arg(norm))
+
+
 def sess_kv_save(kv: torch.Tensor, n_blocks: int, kv_dim: int, max_seq: int, pos: int, path: str,
                  stream=None) -> None:
     """Writes the first pos rows of every block's K and V regions of the device blob kv

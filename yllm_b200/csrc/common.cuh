@@ -34,6 +34,12 @@ DevCtx* dev_ctx(char* err, size_t errlen);   // current device's context (nullpt
 int* noalloc_status_word();
 int dev_num_sms();
 
+// Page sizes of the paged cache (tokens): powers of two, so a tensor copy's box of min(page, tile) rows
+// lies in one page and starts on a 1024-byte swizzle boundary.
+inline bool paged_size_ok(uint32_t page_size) {
+    return page_size >= 16 && page_size <= 256 && (page_size & (page_size - 1)) == 0;
+}
+
 #define YATTN_CHECK_LAUNCH(err, errlen, what)                                            \
     do {                                                                                 \
         cudaError_t e_ = cudaGetLastError();                                             \
@@ -58,6 +64,9 @@ enum : int {
     ST_GDN_TIMEOUT = 301,
     ST_GEMV_TIMEOUT = 501,
     ST_EXCHANGE_TIMEOUT = 401,
+    ST_PAGED_TIMEOUT = 601,
+    ST_PAGED_BAD_PAGE = 602,     // a block table entry or slot outside the pool
+    ST_PAGED_BAD_REQUEST = 603,  // lengths or offsets of a request that contradict the call's arguments
 };
 
 // Upper bound of any spin in these kernels (ns of %globaltimer).  Far above
