@@ -46,8 +46,9 @@ void yattn_clear_error(void);
  * bounded wait that timed out (a kernel that times out returns early instead
  * of hanging), 103 if a decode run met a malformed work item (q or gate
  * not 16-byte aligned; with a pool, K/V not at a row of the pool) and
- * stopped, or 202 if a prefill told YATTN_PREFILL_Q_F16 met a q value that is
- * not an fp16 value.  It covers the allocation-free decode too, whose word sits in its
+ * stopped, 202 if a prefill told YATTN_PREFILL_Q_F16 met a q value that is
+ * not an fp16 value, 602 if a paged-cache call met a page or slot outside the
+ * pool, or 603 if it met a request that contradicts its arguments.  It covers the allocation-free decode too, whose word sits in its
  * static scratch; polling creates neither word.  Synchronises the legacy
  * default stream. */
 int yattn_device_status(int* status_out, int clear, char* err, size_t errlen);
@@ -555,6 +556,37 @@ int yattn_rope_store_kv_paged(void* q_out, uint32_t q_out_stride, const void* q,
                               uint32_t n_kv_heads, uint32_t head_dim, uint32_t kv_dim, int rope_kind,
                               uint32_t n_rope_dims, float theta, const YattnQkNorm* qk_norm, void* stream,
                               char* err, size_t errlen);
+
+/* Causal attention of the requests' new tokens over their paged cache, ragged:
+ * request r's tokens are rows cu_new[r]..cu_new[r+1] of q and out; its keys are
+ * the first kv_len[r] rows of the pages tables[r*table_stride + 0..], the new
+ * tokens' own rows (already stored) included.  New token i of n attends keys
+ * 0..kv_len-n+i; a token with no key to see (kv_len < n) gets zeros.  Query
+ * head hh reads kv head hh/(n_heads/n_kv_heads); scale 1/sqrt(head_dim).  gate
+ * (or NULL): out is multiplied by sigmoid(gate), as yattn_attn_prefill.
+ * q, gate and out hold activations of type `act`, tokens *_stride elements
+ * apart.  Rows from cu_new[n_seqs] on are not written; n_tokens is q's row
+ * count.  max_new is an upper bound of the requests' new tokens (host): up to 8
+ * query rows per kv head (max_new * n_heads/n_kv_heads) run the decode form,
+ * more run 128-row tiles on tcgen05.  Work is divided evenly over the SMs from
+ * the lengths on the device, so nothing here depends on them at capture time.
+ * fp32 activations keep about 22 bits of q and of the softmax weights (fp16 hi
+ * + lo planes); 16-bit activations run one plane of each in the tiles form.
+ * A block table entry outside the pool reads as zero rows (device status 602);
+ * a request whose offsets or lengths contradict the arguments, or which has
+ * more than max_new tokens, is skipped, its rows of out not written (603).
+ * head_dim 64/128/256, n_heads a multiple of n_kv_heads.
+ * workspace: yattn_attn_paged_workspace_bytes, its first 4096 bytes zeroed once; a
+ * call leaves them zero.  Calls that may overlap (other streams, graphs) need
+ * a workspace each; after status 601 zero it again. */
+size_t yattn_attn_paged_workspace_bytes(uint32_t head_dim);
+int yattn_attn_paged(void* out, uint32_t out_stride, const void* q, uint32_t q_stride, const void* gate,
+                     uint32_t gate_stride, int act, const uint16_t* kpool, const uint16_t* vpool,
+                     uint32_t n_pages, uint32_t page_size, const int32_t* tables, uint32_t max_pages,
+                     uint32_t table_stride, const int32_t* cu_new, const int32_t* kv_len, uint32_t n_seqs,
+                     uint32_t n_tokens, uint32_t max_new, uint32_t n_heads, uint32_t n_kv_heads,
+                     uint32_t head_dim, uint32_t kv_dim, void* workspace, size_t workspace_bytes,
+                     void* stream, char* err, size_t errlen);
 
 /* ------------------------------------------------ seeded input generator
  * Deterministic on every device and bit-identical to the CPU restatement in

@@ -1,0 +1,249 @@
+"""Attention over the paged cache against a plain 64-bit form.
+
+Tolerance, per output element o = sum_s p_s v_s / l with p_s = 2^(s_s - m) <= 1 and l >= 1 (64-bit values below):
+  scores  q is a row's power of two times hi + lo fp16 planes: off by 2^-22 of the row's largest |q| (16-bit
+          activations in 128-row tiles: one plane, exact down to 2^-25 of it).  With A = max_s sum_d max|q| |k_sd| /
+          sqrt(hd), a product of hd terms accumulated in fp32 adds hd 2^-24 A, and scale, subtraction of m and the
+          power of two's argument 4 * 2^-24 * 1.45 A: ds = A (2^-22 + 2^-25 + hd 2^-24 + 2^-21).
+  p       relative 2^-22 from ex2.approx and 2^-22 from the hi + lo planes (one plane: 2^-11, the half step of fp16);
+          p is scaled to 2^7 or more at the row's largest, so the planes' subnormals leave 2^-32 absolute.
+  sums    L keys in steps of 16: (L/16 + 16) 2^-24 relative to sum p |v|, and pieces' merges 2^-20.
+So |err| <= V (2 ds + e_p + (L/16) 2^-24 + 2^-20) + 2^-32 sum |v| / l, with V = sum p |v| / l, and a half
+step of the output's type.  A gate's sigmoid (__expf, 2^-20 relative here) multiplies all of it."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+ROWS = 8   # query rows per kv head that the decode form takes
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    torch.cuda.set_device(0)
+    return torch.device("cuda:0")
+
+
+class Case:
+    """Random pages, tables and tokens; rows of the pages that no request owns are NaN."""
+
+    def __init__(self, dev, H, KV, hd, page, lens, new, act="f32", gate=False, seed=0, pad=0, kv_extra=0, q_scale=1.0,
+                 stride_extra=0, width_extra=2):
+        self.geo = (H, KV, hd)
+        self.page, self.lens, self.new = page, [int(x) for x in lens], [int(x) for x in new]
+        g = torch.Generator(device=dev).manual_seed(seed)
+        rng = np.random.default_rng(seed)
+        need = [-(-x // page) for x in self.lens]
+        n_pages = sum(need) + 3
+        kd = KV * hd + kv_extra
+        order = rng.permutation(n_pages)
+        width = max(need + [1]) + width_extra
+        tab = rng.integers(-5, 2 ** 31 - 1, (len(lens), width)).astype(np.int32)   # entries past a request: junk
+        owned = np.zeros(n_pages * page, bool)
+        at = 0
+        self.rows = []
+        for r, m in enumerate(need):
+            tab[r, :m] = order[at:at + m]
+            t = np.arange(self.lens[r])
+            rows = tab[r, t // page].astype(np.int64) * page + t % page
+            owned[rows] = True
+            self.rows.append(torch.from_numpy(rows).to(dev))
+            at += m
+        self.tables = torch.from_numpy(tab).to(dev)
+        owned = torch.from_numpy(owned).to(dev)
+        self.kp, self.vp = (torch.randn(n_pages * page, kd, generator=g, device=dev).half() for _ in range(2))
+        self.kp[~owned] = float("nan")
+        self.vp[~owned] = float("nan")
+        self.total = sum(self.new)
+        T = self.total + pad
+        wide = lambda: torch.randn(T, H * hd + stride_extra, generator=g, device=dev)[:, :H * hd]
+        self.q = (wide() * q_scale).to(DT[act]) if not stride_extra else \
+            torch.randn(T, H * hd + stride_extra, generator=g, device=dev).to(DT[act])[:, :H * hd]
+        self.gate = wide().to(DT[act]) if gate else None
+        self.out = torch.full((T, H * hd + 8), 3.0, dtype=DT[act], device=dev)
+        self.cu = torch.tensor(np.concatenate([[0], np.cumsum(self.new)]).astype(np.int32), device=dev)
+        self.kv = torch.tensor(np.asarray(self.lens, np.int32), device=dev)
+
+    def run(self, max_new=None, out=None, **kw):
+        from yllm_b200 import attn
+        H, KV, hd = self.geo
+        out = self.out if out is None else out
+        attn.attn_paged(out[:, :H * hd], self.q, self.kp.view(-1, self.page, self.kp.shape[1]),
+                        self.vp.view(-1, self.page, self.vp.shape[1]), self.tables, self.cu, self.kv,
+                        max(self.new) if max_new is None else max_new, H, KV, hd, gate=self.gate, **kw)
+
+    def want(self, rows_form):
+        """(values, bounds) in 64 bits for the rows of the requests."""
+        H, KV, hd = self.geo
+        g = H // KV
+        one_plane = not rows_form and self.q.dtype != torch.float32
+        e_p = 2.0 ** -11 + 2.0 ** -22 if one_plane else 2.0 ** -21
+        o = torch.zeros(self.total, H * hd, dtype=torch.float64, device=self.q.device)
+        bar = torch.zeros_like(o)
+        a = 0
+        for r, (L, n) in enumerate(zip(self.lens, self.new)):
+            if n and L:
+                k = self.kp[self.rows[r]][:, :KV * hd].double().view(L, KV, hd).permute(1, 0, 2)
+                v = self.vp[self.rows[r]][:, :KV * hd].double().view(L, KV, hd).permute(1, 0, 2)
+                q = self.q[a:a + n].double().reshape(n, KV, g, hd).permute(1, 2, 0, 3)            # KV g n hd
+                s = torch.einsum("hgnd,hld->hgnl", q, k) / np.sqrt(hd)
+                big = q.abs().amax(-1)                                                             # KV g n
+                A = big * (k.abs().sum(-1).amax(-1) / np.sqrt(hd))[:, None, None]
+                ds = A * (2.0 ** -22 + 2.0 ** -25 + hd * 2.0 ** -24 + 2.0 ** -21)
+                pos = L - n + torch.arange(n, device=s.device)
+                seen = torch.arange(L, device=s.device)[None, :] <= pos[:, None]
+                s = s.masked_fill(~seen, -np.inf)
+                p = torch.exp(s - s.amax(-1, keepdim=True).clamp(min=-1e300))
+                l = p.sum(-1, keepdim=True).clamp(min=1e-300)
+                val = torch.einsum("hgnl,hld->hgnd", p, v) / l
+                V = torch.einsum("hgnl,hld->hgnd", p, v.abs()) / l
+                tail = torch.einsum("nl,hld->hnd", seen.double(), v.abs())[:, None] / l * 2.0 ** -32
+                b = V * (2 * ds[..., None] + e_p + (L / 16 + 16) * 2.0 ** -24 + 2.0 ** -20) + tail
+                dead = (pos < 0)[None, None, :, None]
+                val, b = val.masked_fill(dead, 0.0), b.masked_fill(dead, 0.0)
+                o[a:a + n] = val.permute(2, 0, 1, 3).reshape(n, H * hd)
+                bar[a:a + n] = b.permute(2, 0, 1, 3).reshape(n, H * hd)
+            a += n
+        if self.gate is not None:
+            sg = torch.sigmoid(self.gate[:self.total].double())
+            bar = bar * sg + (o * sg).abs() * 2.0 ** -20
+            o = o * sg
+        dt = self.q.dtype
+        return o, bar + o.abs() * torch.finfo(dt).eps / 2 + (2.0 ** -25 if dt == torch.float16 else 2.0 ** -126)
+
+    def check(self, out=None, max_new=None):
+        torch.cuda.synchronize()
+        from yllm_b200 import attn
+        assert attn.device_status() == 0
+        H, KV, hd = self.geo
+        out = self.out if out is None else out
+        rows_form = (max(self.new) if max_new is None else max_new) * (H // KV) <= ROWS
+        want, bar = self.want(rows_form)
+        got = out[:self.total, :H * hd].double()
+        err = (got - want).abs()
+        assert bool((err <= bar).all()), f"worst {float((err / bar).max()):.3g} of its bar, nan {int(got.isnan().sum())}"
+        assert bool((out[self.total:] == 3.0).all()) and bool((out[:, H * hd:] == 3.0).all())
+
+
+GEO = [(14, 2, 64), (32, 8, 128), (16, 2, 256), (4, 4, 128), (3, 3, 64), (5, 1, 128), (8, 1, 256)]
+
+
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("H,KV,hd", GEO)
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_single_tokens(dev, act, H, KV, hd, page):
+    """One token per request: lengths of one, around pages and blocks, and long enough to be cut."""
+    lens = [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 300, 1000]
+    c = Case(dev, H, KV, hd, page, lens, [1] * len(lens), act=act, gate=(hd == 256), seed=H + hd + page, pad=2,
+             kv_extra=16 if H == 32 else 0)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("lens,new", [
+    ([5000], [1]), ([70000], [1]), ([0, 0, 9], [0, 0, 1]), ([33, 0, 1, 4097], [1, 0, 1, 1]), ([1], [1]),
+])
+@pytest.mark.parametrize("H,KV,hd", [(32, 8, 128), (14, 2, 64), (16, 2, 256)])
+def test_single_tokens_lengths(dev, lens, new, H, KV, hd):
+    c = Case(dev, H, KV, hd, 16, lens, new, seed=sum(lens), pad=1)
+    c.run()
+    c.check()
+    first = c.out.clone()
+    for _ in range(3):   # the pieces are merged in one order: the same bits every time
+        c.out.fill_(3.0)
+        c.run()
+        assert torch.equal(c.out, first)
+
+
+@pytest.mark.parametrize("n", [400, 1000])
+def test_many_requests(dev, n):
+    rng = np.random.default_rng(n)
+    lens = rng.integers(0, 150, n)
+    new = (rng.random(n) < 0.7).astype(int) * (lens > 0)
+    c = Case(dev, 8, 2, 64, 16, lens, new, seed=n)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("H,KV,hd,new", [(8, 4, 128, [4, 1, 3, 2]), (4, 4, 64, [8, 5, 1, 0]), (2, 1, 256, [4, 4, 2, 1])])
+def test_few_tokens_rows_form(dev, H, KV, hd, new):
+    """Several tokens per request with at most 8 rows per kv head: each row has its own last key."""
+    c = Case(dev, H, KV, hd, 32, [4, 700, 65, 2000], new, act="f32", seed=hd)
+    c.run()
+    c.check()
+
+
+def test_token_with_no_key_gets_zeros(dev):
+    """kv_len < new: the first tokens see nothing."""
+    c = Case(dev, 4, 4, 64, 16, [2, 0, 5], [4, 3, 2], seed=9)
+    c.run()
+    c.check()
+    assert bool((c.out[:2, :256] == 0).all()) and bool((c.out[4:7, :256] == 0).all())
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 20, 2.0 ** -30])
+def test_rows_form_far_q(dev, scale):
+    """q far outside fp16's range."""
+    c = Case(dev, 8, 2, 128, 16, [50, 333], [1, 1], seed=4, q_scale=scale)
+    c.run()
+    c.check()
+
+
+# ------------------------------------------------------------- 128-row tiles
+
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("H,KV,hd", GEO)
+@pytest.mark.parametrize("page", [16, 128])
+def test_chunks(dev, act, H, KV, hd, page):
+    """Chunks of odd sizes beside single tokens and requests without any, from an empty cache and behind one."""
+    lens = [40, 1, 129, 700, 0, 65, 257, 300]
+    new = [40, 1, 130 - 1, 33, 0, 1, 2, 100]
+    c = Case(dev, H, KV, hd, page, lens, new, act=act, gate=(hd == 256), seed=H + hd + page, pad=3,
+             stride_extra=16 if page == 128 else 0)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("lens,new", [
+    ([9], [9]), ([128], [128]), ([1000], [1000]), ([5000], [16]), ([40000], [33]), ([17, 16, 15], [17, 16, 15]),
+    ([3, 0, 40], [60, 20, 40]), ([2500, 31, 1], [70, 31, 1]),
+])
+@pytest.mark.parametrize("H,KV,hd", [(32, 8, 128), (14, 2, 64), (16, 2, 256)])
+def test_chunks_lengths(dev, act, lens, new, H, KV, hd):
+    """One request to a few: tiles cut over many CTAs, and tokens that see no key (kv_len < new)."""
+    c = Case(dev, H, KV, hd, 16, lens, new, act=act, seed=sum(lens) + hd, pad=1)
+    c.run()
+    c.check()
+    first = c.out.clone()
+    for _ in range(3):
+        c.out.fill_(3.0)
+        c.run()
+        assert torch.equal(c.out, first)
+
+
+def test_chunks_many_requests(dev):
+    rng = np.random.default_rng(8)
+    n = 500
+    new = np.where(rng.random(n) < 0.1, rng.integers(0, 60, n), 1)
+    lens = new + rng.integers(0, 200, n)
+    c = Case(dev, 8, 2, 128, 32, lens, new, seed=8)
+    c.run()
+    c.check()
+
+
+def test_wide_group_single_tokens(dev):
+    """16 heads per kv head: a single token does not fit the decode form."""
+    c = Case(dev, 32, 2, 128, 16, [1, 16, 777, 3000], [1, 1, 1, 1], seed=2)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("act,scale", [("f32", 2.0 ** 20), ("f32", 2.0 ** -30), ("bf16", 2.0 ** 20)])
+def test_tiles_far_q(dev, act, scale):
+    c = Case(dev, 8, 2, 128, 16, [50, 333], [20, 100], act=act, seed=4, q_scale=scale)
+    c.run()
+    c.check()

@@ -62,3 +62,30 @@ def test_empty_calls_do_nothing():
     err = C.create_string_buffer(512)
     args = list(dict(STORE, n_tokens=0, q=None).values())
     assert _lib.lib.yattn_rope_store_kv_paged(*args, err, 512) == 0
+
+
+ATTN = dict(out=P, out_stride=512, q=P, q_stride=512, gate=None, gate_stride=0, act=0, kpool=P, vpool=P, n_pages=8,
+            page_size=16, tables=P, max_pages=4, table_stride=4, cu_new=P, kv_len=P, n_seqs=2, n_tokens=5, max_new=3,
+            n_heads=4, n_kv=2, head_dim=128, kv_dim=256, ws=P, ws_bytes=1 << 30, stream=None)
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(out=None), "null"), (dict(tables=None), "null"), (dict(act=7), "activation"), (dict(page_size=24), "page_size"),
+    (dict(head_dim=96), "head_dim"), (dict(n_kv=3), "multiple"), (dict(n_heads=0), "multiple"), (dict(n_kv=0), "multiple"),
+    (dict(kv_dim=128), "kv_dim"), (dict(kv_dim=260), "kv_dim"), (dict(q_stride=500), "strides"),
+    (dict(out_stride=514), "strides"), (dict(act=1, q_stride=516), "strides"),
+    (dict(gate=P, gate_stride=256), "strides"), (dict(q=P + 4), "aligned"), (dict(gate=P + 4, gate_stride=512), "aligned"),
+    (dict(ws=P + 8), "aligned"), (dict(cu_new=P + 1), "aligned"), (dict(max_pages=0), "table"),
+    (dict(table_stride=3), "table"), (dict(max_pages=1 << 27, table_stride=1 << 27), "table"), (dict(n_pages=0), "2^31"),
+    (dict(n_pages=1 << 27), "2^31"), (dict(n_seqs=65536), "requests"), (dict(n_tokens=1 << 30), "tokens"),
+    (dict(ws=None), "workspace"), (dict(ws_bytes=4096), "workspace"),
+])
+def test_attn_refuses(change, word):
+    _refused("yattn_attn_paged", list(dict(ATTN, **change).values()), word)
+
+
+@pytest.mark.parametrize("change", [dict(n_seqs=0), dict(n_tokens=0), dict(max_new=0)])
+def test_attn_of_nothing(change):
+    from yllm_b200 import _lib
+    err = C.create_string_buffer(512)
+    assert _lib.lib.yattn_attn_paged(*dict(ATTN, **change).values(), err, 512) == 0

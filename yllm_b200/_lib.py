@@ -162,6 +162,9 @@ PROTOS = {
     "yattn_page_step": (C.c_int, [vp, vp, vp, vp, u32, vp, vp, u32, u32, vp, u32, vp, vp, vp, u32, u32, vp, *E]),
     "yattn_rope_store_kv_paged": (C.c_int, [vp, u32, vp, u32, vp, u32, vp, u32, C.c_int, vp, vp, u64, vp, vp, u32, u32,
                                             u32, u32, u32, C.c_int, u32, C.c_float, vp, vp, *E]),
+    "yattn_attn_paged_workspace_bytes": (sz, [u32]),
+    "yattn_attn_paged": (C.c_int, [vp, u32, vp, u32, vp, u32, C.c_int, vp, vp, u32, u32, vp, u32, u32, vp, vp, u32, u32,
+                                   u32, u32, u32, u32, u32, vp, sz, vp, *E]),
     "yattn_checksum": (C.c_int, [vp, sz, C.POINTER(u64), vp, *E]),
 }
 

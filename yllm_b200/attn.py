@@ -504,6 +504,60 @@ def rope_store_kv_paged(q_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
              theta, _norm_arg(norm))
 
 
+_paged_ws: dict = {}   # (device, stream, head_dim) -> workspace of attn_paged's eager calls on that stream
+
+
+def paged_workspace(head_dim: int, device=None) -> torch.Tensor:
+    """A zeroed workspace for attn_paged, for callers that keep their own (one per stream or graph in flight)."""
+    return torch.zeros(lib.yattn_attn_paged_workspace_bytes(head_dim), dtype=torch.uint8, device=device or "cuda")
+
+
+def _paged_workspace(head_dim: int, dev: int, stream) -> torch.Tensor:
+    """The stream's own workspace: calls on one stream run in order, so they can share it.  A call being captured
+    gets a fresh one (its zeroing is captured too): the graph may be replayed beside other work."""
+    with torch.cuda.device(dev), torch.cuda.stream(stream):
+        if torch.cuda.is_current_stream_capturing():
+            return paged_workspace(head_dim, torch.device("cuda", dev))
+        key = (dev, stream.cuda_stream, head_dim)
+        ws = _paged_ws.get(key)
+        if ws is None:
+            ws = _paged_ws[key] = paged_workspace(head_dim, torch.device("cuda", dev))
+        return ws
+
+
+def attn_paged(out: torch.Tensor, q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, tables: torch.Tensor,
+               cu_new: torch.Tensor, kv_len: torch.Tensor, max_new: int, n_heads: int, n_kv_heads: int, head_dim: int,
+               gate: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, stream=None) -> None:
+    """Causal attention of ragged new tokens (rows cu_new[r]..cu_new[r+1] of q, fp32 / fp16 / bf16) over the first
+    kv_len[r] rows of each request's pages, the new tokens' rows included; max_new bounds a request's new tokens.
+    Rows of out behind the last request stay as they are."""
+    if not q.is_cuda or q.dtype not in _ACT:
+        raise ValueError("q must be a CUDA tensor of float32, float16 or bfloat16")
+    cols = n_heads * head_dim
+    _tokens(q, "q", q, cols)
+    _tokens(out, "out", q, cols)
+    if gate is not None:
+        _tokens(gate, "gate", q, cols)
+    _pools(kpool, vpool, n_kv_heads, head_dim)
+    if kpool.device != q.device:
+        raise ValueError("the pools must be on q's device")
+    _i32_on(q, cu_new=cu_new, kv_len=kv_len)
+    _tables(tables, q)
+    n = kv_len.numel()
+    if cu_new.numel() != n + 1 or tables.shape[0] != n:
+        raise ValueError("cu_new (one more) and tables must have one entry per request of kv_len")
+    if workspace is None:
+        dev = q.device.index
+        workspace = _paged_workspace(head_dim, dev, stream if stream is not None else torch.cuda.current_stream(dev))
+    elif workspace.device != q.device or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous tensor on q's device (paged_workspace)")
+    _call_on("yattn_attn_paged", q, stream, out.data_ptr(), _row_stride(out), q.data_ptr(), _row_stride(q),
+             _ptr(gate), _row_stride(gate) if gate is not None else 0, _ACT[q.dtype], kpool.data_ptr(),
+             vpool.data_ptr(), kpool.shape[0], kpool.shape[1], tables.data_ptr(), tables.shape[1],
+             _table_stride(tables), cu_new.data_ptr(), kv_len.data_ptr(), n, q.shape[0], max_new, n_heads, n_kv_heads,
+             head_dim, kpool.shape[2], workspace.data_ptr(), workspace.numel() * workspace.element_size())
+
+
 def sess_kv_save(kv: torch.Tensor, n_blocks: int, kv_dim: int, max_seq: int, pos: int, path: str,
                  stream=None) -> None:
     """Writes the first pos rows of every block's K and V regions of the device blob kv

@@ -1,0 +1,714 @@
+// paged_tiles.cu -- paged attention of token chunks on tcgen05 / TMEM / TMA: 128-row query tiles.
+//
+// A tile's rows are (token, head of the kv head's group) pairs, token-major, so a kv head's K and V are read
+// once for all its query heads, any group size fills the tile, and one ragged batch may mix long chunks
+// with single tokens.  Math per key block of BN keys, in the log2 domain with a running maximum m:
+//     S = Q K^T,  P = 2^(S c - m),  l = l 2^(m_old - m) + sum P,  O = O 2^(m_old - m) + P V.
+// fp32 activations (PREC): q = hi + lo and P = hi + lo in fp16, four products for about 22 bits.  16-bit
+// activations: one plane of each (fp16 holds their q exactly; P's half step 2^-11 is below the output's own
+// rounding at bf16 and equal to it at fp16).  Each q row is scaled by a power of two into (-2, 2) first,
+// and P carries a factor 2^7 (it cancels in O / l): see row_scale() and kPUp.
+//
+// One persistent CTA per SM walks its share of the schedule (paged.cuh).  Warps:
+//   0-7  softmax: row r of the tile (TMEM lane r) belongs to warps r/32 and r/32 + 4, which halve each
+//        block's columns.  They fetch Q (hi to shared memory, lo to TMEM), turn S into P in place, rescale
+//        O when m grows by more than 2^8, and write the unit's rows or partials.
+//   8, 10  K and V blocks by tensor copies into their rings, a box of min(page, BN) rows x 64 dims per lane.
+//   9    MMA issue.  S runs up to NSB blocks ahead of the softmax.
+//   11   the schedule: units into a ring of four descriptors, so finding the next unit is off the others' path.
+// V rows behind the last key the tile sees hold whatever the page held: the PV product stops at the 16-key
+// step that holds that key, and the rows after it in that step are zeroed in shared memory first.
+#include "paged.cuh"
+#include "tcgen05.cuh"
+
+#include <algorithm>
+
+namespace yattn {
+namespace {
+
+constexpr int BM = static_cast<int>(kPagedTileRows);
+constexpr int kTThreads = 384;
+constexpr int NU = 4;                    // unit descriptors in flight
+// P's factor: m may be stale by 8 binades, and fp16 ends below 2^16
+constexpr float kPUp = 7.f;
+
+template <int HD> struct TCfg {
+    static constexpr int BN = HD >= 256 ? 64 : 128;
+    static constexpr int KST = HD >= 256 ? 2 : 3;           // K ring depth
+    static constexpr int VST = HD >= 128 ? 2 : 3;           // V ring depth: V(j) is needed two blocks after K(j)
+    static constexpr int Q_BYTES = BM * HD * 2;
+    static constexpr int KV_BYTES = BN * HD * 2;
+    static constexpr int OFF_Q = 0;
+    static constexpr int OFF_K = OFF_Q + Q_BYTES;
+    static constexpr int OFF_V = OFF_K + KST * KV_BYTES;
+    static constexpr int OFF_X = OFF_V + VST * KV_BYTES;    // [2 blocks][2 halves][BM] floats: row maxima / sums
+    static constexpr int OFF_U = OFF_X + 2 * 2 * BM * 4;    // [NU] units, 64 B apart
+    static constexpr int OFF_SCRATCH = OFF_U + NU * 64;     // the schedule's sums
+    static constexpr int OFF_BAR = OFF_SCRATCH + 40 * 8;
+    static constexpr int SMEM = OFF_BAR + 320 + 1024;       // + barriers, + alignment slack
+    static constexpr uint32_t TMEM_COLS = 512;
+    static constexpr uint32_t COL_S = 0;                    // S buffer b at [b*BN, (b+1)*BN)
+    static constexpr uint32_t COL_O = 3 * BN;
+    static_assert(3 * BN + HD <= static_cast<int>(TMEM_COLS), "TMEM columns");
+    // Q_lo (PREC), HD/2 columns: after O at head_dim 64, in the third S buffer (then after O) above
+    static constexpr int NSB_LO = HD == 64 ? 3 : 2;
+    __host__ __device__ static constexpr uint32_t qlo_col(int kk) {
+        return HD == 64 ? COL_O + HD + 8u * kk
+             : HD == 128 ? 2u * BN + 8u * kk
+             : (kk < 8 ? 2u * BN + 8u * kk : COL_O + HD + 8u * (kk - 8));
+    }
+    static_assert(qlo_col(HD / 16 - 1) + 8 <= TMEM_COLS, "Q_lo columns");
+    static_assert(SMEM <= 232448 && sizeof(PagedUnit) <= 64, "shared memory");
+};
+
+template <int KST, int VST> struct TBars {
+    uint64_t k_full[KST], k_empty[KST], v_full[VST], v_empty[VST];
+    uint64_t s_full[3], p_full[3], pv_done[3];   // per S buffer
+    uint64_t o_done, q_full, mma_drain;
+    uint64_t u_full[NU], u_empty[NU];
+    uint32_t tmem_base;
+    int abort_flag, last_flag;
+};
+
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+
+template <int HD, bool PREC>
+__global__ void __launch_bounds__(kTThreads, 1)
+    k_paged_tiles(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const __grid_constant__ PagedParams p) {
+    using C = TCfg<HD>;
+    constexpr int BN = C::BN, HB = BN / 2, KST = C::KST, VST = C::VST, NPAN = HD / 64;
+    constexpr uint32_t NSB = PREC ? C::NSB_LO : 3;
+    using Sched = PagedSched<BN, BM>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sQ = smem + C::OFF_Q;
+    uint8_t* sK = smem + C::OFF_K;
+    uint8_t* sV = smem + C::OFF_V;
+    float* xch = reinterpret_cast<float*>(smem + C::OFF_X);
+    using Bars = TBars<KST, VST>;
+    static_assert(sizeof(Bars) <= 320, "barriers");
+    Bars* bars = reinterpret_cast<Bars*>(smem + C::OFF_BAR);
+    volatile int* abort_flag = &bars->abort_flag;
+    auto unit_at = [&](uint32_t i) { return reinterpret_cast<PagedUnit*>(smem + C::OFF_U + (i % NU) * 64); };
+    int* const status = p.status;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < KST; ++s) {
+            mbar_init(&bars->k_full[s], 1);
+            mbar_init(&bars->k_empty[s], 1);
+        }
+        for (int s = 0; s < VST; ++s) {
+            mbar_init(&bars->v_full[s], 1);
+            mbar_init(&bars->v_empty[s], 1);
+        }
+        for (int s = 0; s < 3; ++s) {
+            mbar_init(&bars->s_full[s], 1);
+            mbar_init(&bars->p_full[s], 8);
+            mbar_init(&bars->pv_done[s], 1);
+        }
+        mbar_init(&bars->o_done, 1);
+        mbar_init(&bars->q_full, 8);
+        mbar_init(&bars->mma_drain, 1);
+        for (int s = 0; s < NU; ++s) {
+            mbar_init(&bars->u_full[s], 1);
+            mbar_init(&bars->u_empty[s], 11);    // K, V, MMA and eight softmax warps
+        }
+        bars->abort_flag = 0;
+        fence_mbar_init();
+    }
+    Sched sched(p);
+    if (!sched.locate(reinterpret_cast<long long*>(smem + C::OFF_SCRATCH))) return;   // the whole block
+    if (warp == 0) tmem_alloc(&bars->tmem_base, C::TMEM_COLS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bars->tmem_base;
+
+    // Unit ui of the list, for one warp: waits for its descriptor.  false: the list has ended (or a wait gave up).
+    auto get_unit = [&](uint32_t ui, PagedUnit& u) -> bool {
+        if (!warp_wait_bounded(&bars->u_full[ui % NU], (ui / NU) & 1u, status, ST_PAGED_TIMEOUT, abort_flag)) return false;
+        u = *unit_at(ui);
+        return !u.done;
+    };
+    auto put_unit = [&](uint32_t ui) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->u_empty[ui % NU]);
+    };
+    // keys the tile's last row sees
+    auto unit_keys = [&](const PagedUnit& u) -> int32_t { return Sched::keys(p, PagedReq{u.tok0, u.n, u.len}, u.j); };
+
+    if (warp == 11) {
+        // ================= schedule =================
+        uint32_t ui = 0;
+        bool ok = true, more = true;
+        while (ok && more) {
+            PagedUnit u;
+            more = sched.next(u);
+            if (ui >= NU)
+                ok = warp_wait_bounded(&bars->u_empty[ui % NU], ((ui / NU) & 1u) ^ 1u, status, ST_PAGED_TIMEOUT, abort_flag);
+            if (ok && lane == 0) {
+                u.done = more ? 0u : 1u;
+                *unit_at(ui) = u;
+                mbar_arrive(&bars->u_full[ui % NU]);
+            }
+            ++ui;
+        }
+    } else if (warp == 8 || warp == 10) {
+        // ================= K / V copies =================
+        const bool is_v = warp == 10;
+        const CUtensorMap* map = is_v ? &tmV : &tmK;
+        uint8_t* ring = is_v ? sV : sK;
+        uint64_t* full = is_v ? bars->v_full : bars->k_full;
+        uint64_t* empty = is_v ? bars->v_empty : bars->k_empty;
+        const uint32_t depth = is_v ? VST : KST;
+        if (lane == 0) prefetch_tensormap(map);
+        const uint32_t page = 1u << p.page_shift, box = min(page, static_cast<uint32_t>(BN));
+        const uint32_t i_pg = lane / NPAN, i_pan = lane % NPAN;   // this lane's box of a block (16 at most)
+        const bool mine = i_pg < BN / box;
+        uint32_t s = 0, ph = 0, issued = 0;                       // ring stage, its pass's parity, blocks in all
+        bool ok = true;
+        PagedUnit u;
+        for (uint32_t ui = 0; ok && get_unit(ui, u); ++ui) {
+            const uint32_t kend = static_cast<uint32_t>(unit_keys(u));
+            const int32_t x = static_cast<int32_t>(u.g * HD + i_pan * 64);
+            auto row_of = [&](uint32_t b) -> int32_t {
+                const uint32_t key = b * BN + i_pg * box;
+                if (!mine || key >= kend) return -1;
+                return paged_row(p, u.r, key >> p.page_shift) + static_cast<int32_t>(key & (page - 1));
+            };
+            int32_t row = u.kb1 > u.kb0 ? row_of(u.kb0) : -1;
+            for (uint32_t b = u.kb0; b < u.kb1; ++b) {
+                if (issued >= depth &&
+                    !warp_wait_bounded(&empty[s], ph ^ 1u, status, ST_PAGED_TIMEOUT, abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t n_copy = __popc(__ballot_sync(0xffffffffu, row >= 0));
+                if (lane == 0) mbar_arrive_expect_tx(&full[s], n_copy * box * 128);
+                __syncwarp();
+                if (row >= 0)
+                    tma_load_2d(ring + s * C::KV_BYTES + i_pan * (BN * 128) + i_pg * (box * 128), map, x, row, &full[s]);
+                ++issued;
+                if (++s == depth) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+                row = b + 1 < u.kb1 ? row_of(b + 1) : -1;
+            }
+            put_unit(ui);
+        }
+        // no copy may still be landing when the CTA exits
+        volatile int dummy = 0;
+        for (uint32_t b = issued > depth ? issued - depth : 0; b < issued; ++b)
+            mbar_wait_bounded(&full[b % depth], (b / depth) & 1u, status, ST_PAGED_TIMEOUT, &dummy);
+    } else if (warp == 9) {
+        // ================= MMA =================
+        constexpr uint32_t IDESC_QK = idesc_f16(BM, BN, 0);
+        constexpr uint32_t IDESC_PV = idesc_f16(BM, HD, 1);
+        // an operand at base + off has the base's descriptor + off / 16
+        const uint64_t dq0 = sdesc_sw128(sQ, 16, 1024);
+        const uint64_t dk0 = sdesc_sw128(sK, 16, 1024);
+        const uint64_t dv0 = sdesc_sw128(sV, BN * 128, 1024);
+        uint32_t ks = 0, kph = 0, vs = 0, vph = 0;      // ring stages and parities
+        uint32_t s_sb = 0, pv_sb = 0, pv_ph = 0;        // S buffer of the next S product, of the next PV product
+        uint32_t qph = 0;
+        bool ok = true;
+        PagedUnit u;
+        for (uint32_t ui = 0; ok && get_unit(ui, u); ++ui) {
+            const uint32_t nb = u.kb1 - u.kb0;
+            if (nb == 0) {
+                put_unit(ui);
+                continue;
+            }
+            const int32_t kend = unit_keys(u);
+            ok = warp_wait_bounded(&bars->q_full, qph, status, ST_PAGED_TIMEOUT, abort_flag);
+            qph ^= 1u;
+            tc_fence_after();
+            // S = Q K^T of the next block into the next S buffer; that buffer's last P was consumed by a PV product
+            // issued earlier, and the tensor core runs one thread's MMAs in order
+            auto do_s = [&]() -> bool {
+                if (!warp_wait_bounded(&bars->k_full[ks], kph, status, ST_PAGED_TIMEOUT, abort_flag)) return false;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint64_t dk = dk0 + ((ks * C::KV_BYTES) >> 4);
+                    const uint32_t d = tmem + C::COL_S + s_sb * BN;
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk) {
+                        const uint64_t a = dq0 + (((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4);
+                        const uint64_t b = dk + (((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
+                        umma_f16(d, a, b, IDESC_QK, kk > 0 ? 1u : 0u);
+                    }
+                    if constexpr (PREC) {   // + Q_lo K^T, A from TMEM
+#pragma unroll
+                        for (int kk = 0; kk < HD / 16; ++kk) {
+                            const uint64_t b = dk + (((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
+                            umma_f16_ts(d, tmem + C::qlo_col(kk), b, IDESC_QK, 1u);
+                        }
+                    }
+                    umma_commit(&bars->s_full[s_sb]);
+                    umma_commit(&bars->k_empty[ks]);
+                }
+                __syncwarp();
+                if (++s_sb == NSB) s_sb = 0;
+                if (++ks == KST) {
+                    ks = 0;
+                    kph ^= 1u;
+                }
+                return true;
+            };
+            // O += P V: keys [16 kk, +16) of a plane are the 8 columns at 32 (kk/2) + 16 plane + 8 (kk%2)
+            auto do_pv = [&](uint32_t jj) -> bool {
+                if (!warp_wait_bounded(&bars->p_full[pv_sb], pv_ph, status, ST_PAGED_TIMEOUT, abort_flag) ||
+                    !warp_wait_bounded(&bars->v_full[vs], vph, status, ST_PAGED_TIMEOUT, abort_flag))
+                    return false;
+                tc_fence_after();
+                const int valid = min(BN, kend - static_cast<int32_t>((u.kb0 + jj) * BN));   // >= 1
+                const int steps = (valid + 15) >> 4;
+                if (valid & 15) {   // the rest of the last 16-key step
+                    const int zrows = steps * 16 - valid;
+                    for (int i = lane; i < zrows * NPAN * 8; i += 32) {
+                        const int row = valid + i / (NPAN * 8), c = i % (NPAN * 8);
+                        *reinterpret_cast<uint4*>(sV + vs * C::KV_BYTES + (c >> 3) * (BN * 128) + row * 128 + (c & 7) * 16) =
+                            make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                if (lane == 0) {
+                    const uint32_t pcol = tmem + C::COL_S + pv_sb * BN;
+                    const uint64_t dv = dv0 + ((vs * C::KV_BYTES) >> 4);
+#pragma unroll
+                    for (int plane = 0; plane < (PREC ? 2 : 1); ++plane)
+#pragma unroll
+                        for (int kk = 0; kk < BN / 16; ++kk)
+                            if (kk < steps)
+                                umma_f16_ts(tmem + C::COL_O, pcol + 32 * (kk >> 1) + 16 * plane + 8 * (kk & 1),
+                                            dv + ((kk * 16 * 128) >> 4), IDESC_PV,
+                                            (jj > 0 || plane > 0 || kk > 0) ? 1u : 0u);
+                    umma_commit(&bars->v_empty[vs]);
+                    umma_commit(&bars->pv_done[pv_sb]);
+                }
+                __syncwarp();
+                if (++pv_sb == NSB) {
+                    pv_sb = 0;
+                    pv_ph ^= 1u;
+                }
+                if (++vs == VST) {
+                    vs = 0;
+                    vph ^= 1u;
+                }
+                return true;
+            };
+            for (uint32_t jj = 0; ok && jj < nb && jj < NSB; ++jj) ok = do_s();
+            for (uint32_t jj = 0; ok && jj < nb; ++jj) {
+                ok = do_pv(jj);
+                if (ok && jj + NSB < nb) ok = do_s();
+            }
+            if (ok && lane == 0) umma_commit(&bars->o_done);
+            put_unit(ui);
+        }
+        // every MMA issued so far completes before TMEM is freed
+        if (lane == 0) {
+            umma_commit(&bars->mma_drain);
+            volatile int dummy = 0;
+            mbar_wait_bounded(&bars->mma_drain, 0, status, ST_PAGED_TIMEOUT, &dummy);
+        }
+        __syncwarp();
+    } else {
+        // ================= softmax warps 0-7 =================
+        const int qd = warp & 3, h = warp >> 2;          // TMEM lane quadrant, half of each block's columns
+        const int r = qd * 32 + lane;                    // row of the tile
+        const uint32_t trow = tmem + (static_cast<uint32_t>(qd * 32) << 16);
+        uint32_t sb = 0, sph = 0, pb = 0, pph = 0;       // S buffer of this block / of the last one, and parities
+        uint32_t oph = 0;
+        // Waits' results are ANDed over the warps that meet at the next barrier, so all of them leave together.
+        for (uint32_t ui = 0;; ++ui) {
+            PagedUnit u;
+            const bool got = get_unit(ui, u);
+            if (!named_bar_and(5, 256, got)) break;      // the end, or a wait that gave up
+            const uint32_t nb = u.kb1 - u.kb0;
+            const uint32_t row0 = u.j * BM, rows = min(static_cast<uint32_t>(BM), static_cast<uint32_t>(u.n) * p.group - row0);
+            const bool live = static_cast<uint32_t>(r) < rows;
+            const bool work = static_cast<uint32_t>(qd * 32) < rows;      // this warp has a live row
+            const uint32_t f = row0 + min(static_cast<uint32_t>(r), rows - 1);
+            const uint32_t tk = f / p.group;
+            const size_t tok = u.tok0 + static_cast<size_t>(tk);
+            const size_t col0 = static_cast<size_t>(u.g * p.group + f % p.group) * HD + h * (HD / 2);
+            const int32_t qpos = u.len - u.n + static_cast<int32_t>(tk);   // last key this row sees
+            const int32_t qpos_min = u.len - u.n + static_cast<int32_t>(row0 / p.group);
+            auto write_out = [&](int c, const float (&x)[32]) {             // columns [c, c + 32) of this half
+                if (!live) return;
+                float y[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) y[i] = x[i];
+                if (p.gate) {
+                    const size_t gi = tok * p.gate_stride + col0 + c;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 g = ld_act2(p.gate, gi + i, p.act);
+                        y[i] *= sigmoid_of(g.x);
+                        y[i + 1] *= sigmoid_of(g.y);
+                    }
+                }
+                const size_t oi = tok * p.out_stride + col0 + c;
+                if constexpr (PREC) {
+                    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + oi);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dst[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+                } else {
+                    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + oi);
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if (p.act == YATTN_ACT_F16) {
+                            w[i] = h2_bits(__floats2half2_rn(y[2 * i], y[2 * i + 1]));
+                        } else {
+                            const __nv_bfloat162 b = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
+                            w[i] = *reinterpret_cast<const uint32_t*>(&b);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                }
+            };
+            if (nb == 0) {                               // no key to see
+                float z[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) z[i] = 0.f;
+#pragma unroll 1
+                for (int c = 0; c < HD / 2; c += 32) write_out(c, z);
+                put_unit(ui);
+                continue;
+            }
+
+            // ---- Q: this thread's half row, scaled by the row's power of two ----
+            float up = 1.f;
+            bool ok = true;
+            {
+                constexpr int CH = HD / 2 < 64 ? HD / 2 : 64;             // columns in registers at a time
+                float x[CH];
+                const size_t qi = tok * p.q_stride + col0;
+                auto load = [&](int c) {
+#pragma unroll
+                    for (int i = 0; i < CH; ++i) x[i] = 0.f;
+                    if (!live) return;
+                    if constexpr (PREC) {
+                        const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + qi + c);
+#pragma unroll
+                        for (int i = 0; i < CH / 4; ++i) {
+                            const float4 v = __ldg(src + i);
+                            x[4 * i] = v.x;
+                            x[4 * i + 1] = v.y;
+                            x[4 * i + 2] = v.z;
+                            x[4 * i + 3] = v.w;
+                        }
+                    } else {
+                        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + qi + c);
+#pragma unroll
+                        for (int i = 0; i < CH / 8; ++i) {
+                            const uint4 v = __ldg(src + i);
+                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const float2 t = p.act == YATTN_ACT_F16
+                                                     ? h2f2(w[k])
+                                                     : make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+                                x[8 * i + 2 * k] = t.x;
+                                x[8 * i + 2 * k + 1] = t.y;
+                            }
+                        }
+                    }
+                };
+                float mx = 0.f;
+#pragma unroll 1
+                for (int c = HD / 2 - CH; c >= 0; c -= CH) {              // ends with columns [0, CH) in x
+                    load(c);
+#pragma unroll
+                    for (int i = 0; i < CH; ++i) mx = fmaxf(mx, fabsf(x[i]));
+                }
+                xch[h * BM + r] = mx;
+                named_bar_sync(1 + qd, 64);                               // the row's two halves
+                mx = fmaxf(xch[r], xch[BM + r]);
+                named_bar_sync(1 + qd, 64);                               // read before the first block's maxima
+                float down;
+                row_scale(mx, down, up);
+#pragma unroll 1
+                for (int c = 0; c < HD / 2; c += CH) {
+                    if (c > 0) load(c);
+                    const int d0 = h * (HD / 2) + c;
+#pragma unroll
+                    for (int i = 0; i < CH; i += 32) {
+                        uint32_t hi[16], lo[16];
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) {
+                            const float a = x[i + 2 * k] * down, b = x[i + 2 * k + 1] * down;
+                            const __half2 hv = __floats2half2_rn(a, b);
+                            hi[k] = h2_bits(hv);
+                            const float2 fv = __half22float2(hv);
+                            lo[k] = h2_bits(__floats2half2_rn(a - fv.x, b - fv.y));
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            *reinterpret_cast<uint4*>(sQ + sw128_offset(r, d0 + i + 8 * k, BM)) =
+                                make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
+                        if constexpr (PREC) tmem_st16(trow + C::qlo_col((d0 + i) / 16), lo);
+                    }
+                }
+                if constexpr (PREC) tmem_wait_st();
+                fence_proxy_async_smem();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->q_full);
+            }
+            const float sl2 = p.scale_log2 * up;
+            float m_run = -INFINITY, l_run = 0.f;        // log2 units; l_run: this half's columns
+            for (uint32_t j = 0; j < nb; ++j) {
+                const bool have = warp_wait_bounded(&bars->s_full[sb], sph, status, ST_PAGED_TIMEOUT, abort_flag);
+                if (!work) {                             // no live row: P's lanes stay as they are, nothing reads them
+                    if (!named_bar_and(1 + qd, 64, have)) {
+                        ok = false;
+                        break;
+                    }
+                } else {
+                    const uint32_t scol = trow + C::COL_S + sb * BN + h * HB;
+                    float sv[HB];
+                    if (have) {
+                        tc_fence_after();
+#pragma unroll
+                        for (int c = 0; c < HB / 32; ++c) {
+                            uint32_t rr[32];
+                            tmem_ld32(scol + c * 32, rr);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) sv[c * 32 + i] = __uint_as_float(rr[i]);
+                        }
+                        tmem_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < HB; ++c) sv[c] = -INFINITY;
+                    }
+                    // causal mask; also drops the stale rows behind the last key (their S may be NaN)
+                    const int32_t kbase = static_cast<int32_t>((u.kb0 + j) * BN) + h * HB;
+                    if (static_cast<int32_t>((u.kb0 + j + 1) * BN) - 1 > qpos_min) {
+#pragma unroll
+                        for (int c = 0; c < HB; ++c)
+                            if (kbase + c > qpos) sv[c] = -INFINITY;
+                    }
+                    float mx4[4] = {sv[0], sv[1], sv[2], sv[3]};
+#pragma unroll
+                    for (int c = 4; c < HB; c += 4) {
+                        mx4[0] = fmaxf(mx4[0], sv[c]);
+                        mx4[1] = fmaxf(mx4[1], sv[c + 1]);
+                        mx4[2] = fmaxf(mx4[2], sv[c + 2]);
+                        mx4[3] = fmaxf(mx4[3], sv[c + 3]);
+                    }
+                    float* xb = xch + (j & 1) * (2 * BM);
+                    xb[h * BM + r] = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                    if (!named_bar_and(1 + qd, 64, have)) {
+                        ok = false;
+                        break;
+                    }
+                    const float mx = fmaxf(xb[r], xb[BM + r]) * sl2;
+                    const float m_new = fmaxf(m_run, mx);
+                    const bool grow = m_new > m_run + 8.0f;          // a stale m costs nothing up to 2^8
+                    const float m_use = grow ? m_new : m_run;
+                    const float alpha = grow ? ex2_approx(m_run - m_use) : 1.0f;
+                    const float m_sub = (m_use == -INFINITY ? 0.f : m_use) - kPUp;   // no key yet: p = 0
+                    const float2 sl2x2 = make_float2(sl2, sl2), negm = make_float2(-m_sub, -m_sub);
+                    const float2 neg1 = make_float2(-1.f, -1.f);
+                    float2 rs2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                    for (int c = 0; c < HB / 32; ++c) {   // 32 keys: 16 columns of P hi, then 16 of P lo
+                        uint32_t hi[16], lo[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float2 x = __ffma2_rn(make_float2(sv[c * 32 + 2 * i], sv[c * 32 + 2 * i + 1]), sl2x2, negm);
+                            const float2 pp = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                            rs2[i & 1] = __fadd2_rn(rs2[i & 1], pp);
+                            const __half2 hv = __floats2half2_rn(pp.x, pp.y);
+                            hi[i] = h2_bits(hv);
+                            if constexpr (PREC) {
+                                const float2 d = __ffma2_rn(__half22float2(hv), neg1, pp);
+                                lo[i] = h2_bits(__floats2half2_rn(d.x, d.y));
+                            }
+                        }
+                        tmem_st16(scol + c * 32, hi);
+                        if constexpr (PREC) tmem_st16(scol + c * 32 + 16, lo);
+                    }
+                    l_run = l_run * alpha + ((rs2[0].x + rs2[0].y) + (rs2[1].x + rs2[1].y));
+                    m_run = m_use;
+                    // ---- O rescale (rare), this half's columns: the last block's PV must have finished.  Both
+                    // halves of the rows see the same `grow`. ----
+                    if (j >= 1 && __any_sync(0xffffffffu, grow)) {
+                        const bool done = warp_wait_bounded(&bars->pv_done[pb], pph, status, ST_PAGED_TIMEOUT, abort_flag);
+                        if (!named_bar_and(1 + qd, 64, done)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < HD / 64; ++c) {
+                            const uint32_t oc = trow + C::COL_O + h * (HD / 2) + c * 32;
+                            uint32_t rr[32];
+                            tmem_ld32(oc, rr);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) rr[i] = __float_as_uint(__uint_as_float(rr[i]) * alpha);
+                            tmem_st32(oc, rr);
+                        }
+                    }
+                    tmem_wait_st();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->p_full[sb]);
+                pb = sb;
+                pph = sph;
+                if (++sb == NSB) {
+                    sb = 0;
+                    sph ^= 1u;
+                }
+            }
+            // ---- the unit's rows: the slot that block nb-1 did not use is free (both halves have read it) ----
+            ok = ok && warp_wait_bounded(&bars->o_done, oph, status, ST_PAGED_TIMEOUT, abort_flag);
+            oph ^= 1u;
+            float* xl = xch + (nb & 1) * (2 * BM);
+            xl[h * BM + r] = l_run;
+            if (!named_bar_and(5, 256, ok)) break;       // every softmax warp
+            tc_fence_after();
+            const float l_row = xl[r] + xl[BM + r];
+            named_bar_sync(1 + qd, 64);                  // read before the next unit's Q maxima
+            const uint32_t ocol = trow + C::COL_O + h * (HD / 2);
+            if (u.n_pieces == 1) {
+                const float inv = l_row == 0.f ? 0.f : 1.0f / l_row;
+#pragma unroll 1
+                for (int c = 0; c < HD / 2; c += 32) {
+                    uint32_t rr[32];
+                    tmem_ld32(ocol + c, rr);
+                    tmem_wait_ld();
+                    float x[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(rr[i]) * inv;
+                    write_out(c, x);
+                }
+                tc_fence_before();
+                put_unit(ui);
+                continue;
+            }
+            // ---- a piece: (m, l, o), o by column quads so that a warp's stores are whole lines ----
+            const int quad0 = h * (HD / 8);              // this half's first column quad
+            auto quads = [&](uint32_t slot) {
+                return reinterpret_cast<float4*>(p.part_o) + (static_cast<size_t>(slot) * (HD / 4) + quad0) * BM + r;
+            };
+            if (h == 0) *reinterpret_cast<float2*>(&p.part_ml[(static_cast<size_t>(u.slot) * BM + r) * 2]) = make_float2(m_run, l_row);
+            float4* po = quads(u.slot);
+#pragma unroll 1
+            for (int c = 0; c < HD / 2; c += 32) {
+                uint32_t rr[32];
+                tmem_ld32(ocol + c, rr);
+                tmem_wait_ld();
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        po[(c / 4 + i) * BM] = make_float4(__uint_as_float(rr[4 * i]), __uint_as_float(rr[4 * i + 1]),
+                                                           __uint_as_float(rr[4 * i + 2]), __uint_as_float(rr[4 * i + 3]));
+                }
+            }
+            tc_fence_before();
+            __threadfence();
+            named_bar_sync(5, 256);
+            if (threadIdx.x == 0)
+                bars->last_flag = atomicInc(&p.counters[u.c_first], u.n_pieces - 1) == u.n_pieces - 1;
+            named_bar_sync(5, 256);
+            if (bars->last_flag && live) {               // the last piece to arrive merges them, in piece order
+                __threadfence();
+                auto ml_of = [&](uint32_t i) {
+                    return __ldcg(reinterpret_cast<const float2*>(
+                        &p.part_ml[(static_cast<size_t>(piece_slot(u.c_first, i)) * BM + r) * 2]));
+                };
+                float M = -INFINITY, l = 0.f;
+                for (uint32_t i = 0; i < u.n_pieces; ++i) M = fmaxf(M, ml_of(i).x);
+                for (uint32_t i = 0; i < u.n_pieces; ++i) {
+                    const float2 ml = ml_of(i);
+                    l += (ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - M)) * ml.y;
+                }
+                const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll 1
+                for (int c = 0; c < HD / 2; c += 32) {
+                    float x[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] = 0.f;
+#pragma unroll 2
+                    for (uint32_t i = 0; i < u.n_pieces; ++i) {
+                        const float4* src = quads(piece_slot(u.c_first, i)) + (c / 4) * BM;
+                        float4 o[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) o[k] = __ldcg(src + k * BM);
+                        const float mi = ml_of(i).x;
+                        const float w = mi == -INFINITY ? 0.f : ex2_approx(mi - M) * inv;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            x[4 * k] += w * o[k].x;
+                            x[4 * k + 1] += w * o[k].y;
+                            x[4 * k + 2] += w * o[k].z;
+                            x[4 * k + 3] += w * o[k].w;
+                        }
+                    }
+                    write_out(c, x);
+                }
+            }
+            put_unit(ui);
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 0) tmem_dealloc(tmem, C::TMEM_COLS);
+}
+
+template <int HD, bool PREC>
+int launch(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, uint32_t ctas, cudaStream_t st,
+           char* err, size_t errlen) {
+    using C = TCfg<HD>;
+    static bool attr_done[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && !attr_done[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(k_paged_tiles<HD, PREC>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e != cudaSuccess) {
+            set_err(err, errlen, "attn_paged: smem attribute (%d bytes): %s", C::SMEM, cudaGetErrorString(e));
+            return -1;
+        }
+        attr_done[dev] = true;
+    }
+    k_paged_tiles<HD, PREC><<<ctas, kTThreads, C::SMEM, st>>>(mk, mv, p);
+    YATTN_CHECK_LAUNCH(err, errlen, "attn_paged");
+    return 0;
+}
+
+}  // namespace
+
+int paged_tiles(const PagedParams& pp, const uint16_t* kpool, const uint16_t* vpool, uint64_t n_rows, uint32_t kv_dim,
+                uint32_t hd, uint32_t n_kv, cudaStream_t st, char* err, size_t errlen) {
+    PagedParams p = pp;
+    p.hc = 1;
+    p.n_groups = n_kv;
+    const uint32_t bn = hd >= 256 ? 64 : 128, box = std::min(1u << p.page_shift, bn);
+    CUtensorMap mk, mv;
+    if (encode_kv_map(&mk, kpool, kv_dim, n_rows, box, err, errlen) ||
+        encode_kv_map(&mv, vpool, kv_dim, n_rows, box, err, errlen))
+        return -1;
+    const uint32_t ctas = std::min<uint32_t>(static_cast<uint32_t>(dev_num_sms()), kPagedMaxPieces);
+    const bool prec = p.act == YATTN_ACT_F32;
+    switch (hd) {
+        case 64: return prec ? launch<64, true>(p, mk, mv, ctas, st, err, errlen)
+                             : launch<64, false>(p, mk, mv, ctas, st, err, errlen);
+        case 128: return prec ? launch<128, true>(p, mk, mv, ctas, st, err, errlen)
+                              : launch<128, false>(p, mk, mv, ctas, st, err, errlen);
+        default: return prec ? launch<256, true>(p, mk, mv, ctas, st, err, errlen)
+                             : launch<256, false>(p, mk, mv, ctas, st, err, errlen);
+    }
+}
+
+}  // namespace yattn
