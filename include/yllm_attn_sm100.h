@@ -541,8 +541,7 @@ int yattn_page_step(int32_t* kv_len_out, int32_t* cu_new, int32_t* slots, int32_
  * the engine's f32_to_f16.  q, k, v and q_out hold activations of type `act`
  * (YATTN_ACT_*), heads contiguous, tokens *_stride elements apart (so q, k and
  * v may be columns of one projection output); q_out may be q itself with the
- * same stride.  A token with slot < 0 is skipped: its rows are neither read
- * nor written.  A slot outside the pool's n_rows rows is not stored and sets
+ * same stride.  A token with slot < 0 is skipped: nothing of it is written.  A slot outside the pool's n_rows rows is not stored and sets
  * device status 602.  Two tokens with one slot: either may remain.
  * rope_kind, n_rope_dims (kind 2: a multiple of 16) and qk_norm as
  * yattn_rope_store_kv, but the angle position*theta^(-2j/n) is taken in 64

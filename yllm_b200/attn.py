@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import threading
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -407,54 +408,82 @@ _ACT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # YATTN_ACT_*
 _F16_BITS = (torch.float16, torch.uint16, torch.int16)
 
 
-def _call_on(name: str, t: torch.Tensor, stream, *args) -> None:
-    """call() on t's device: the given stream of it, or its current one."""
-    dev = t.device.index
+_tls = threading.local()   # err: this thread's message buffer
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _call_on(name: str, dev: int, stream, *args) -> None:
+    """call() on device dev, on the given stream of it or its current one.  One message buffer per thread: the
+    library writes it on failure only."""
     if stream is None:
-        stream = torch.cuda.current_stream(dev)
-    elif stream.device_index != dev:
+        raw = _raw_stream(dev)
+    elif stream.device_index == dev:
+        raw = stream.cuda_stream
+    else:
         raise ValueError(f"{name}: the stream is on cuda:{stream.device_index}, the tensors on cuda:{dev}")
+    try:
+        err = _tls.err
+    except AttributeError:
+        err = _tls.err = C.create_string_buffer(512)
     if dev == torch.cuda.current_device():
-        call(name, *args, stream.cuda_stream)
+        rc = getattr(lib, name)(*args, raw, err, 512)
     else:
         with torch.cuda.device(dev):
-            call(name, *args, stream.cuda_stream)
+            rc = getattr(lib, name)(*args, raw, err, 512)
+    if rc != 0:
+        raise _lib.YattnError(f"{name}: {err.value.decode(errors='replace')}")
 
 
-def _i32_on(ref: torch.Tensor, **tensors: torch.Tensor) -> None:
-    for name, t in tensors.items():
-        if t.dtype != torch.int32 or t.device != ref.device or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 tensor on {ref.device}")
+def _i32_on(dev: int, names: str, *tensors: torch.Tensor) -> None:
+    i32 = torch.int32
+    for i, t in enumerate(tensors):
+        if t.dtype is not i32 or t.get_device() != dev or not t.is_contiguous():
+            raise ValueError(f"{names.split()[i]} must be a contiguous int32 tensor on cuda:{dev}")
 
 
-def _tables(tables: torch.Tensor, ref: torch.Tensor) -> None:
-    if (tables.dtype != torch.int32 or tables.device != ref.device or tables.dim() != 2 or tables.shape[1] == 0
-            or tables.stride(1) != 1 or (tables.shape[0] > 1 and tables.stride(0) < tables.shape[1])):
-        raise ValueError(f"tables must be an int32 [requests, pages] tensor on {ref.device} with contiguous rows")
+def _table_shape(tables: torch.Tensor, dev: int, n: int) -> tuple:
+    """(pages per row, row stride) of a block table of n requests."""
+    if tables.dtype is torch.int32 and tables.get_device() == dev and tables.dim() == 2:
+        rows, width = tables.shape
+        stride, one = tables.stride()
+        if rows == 1 and width > 0:
+            stride = width
+        if rows == n and width > 0 and (one == 1 or width == 1) and stride >= width:
+            return width, stride
+    raise ValueError(f"tables must be an int32 [{n} requests, pages] tensor on cuda:{dev} with contiguous rows")
 
 
-def _table_stride(tables: torch.Tensor) -> int:
-    return tables.stride(0) if tables.shape[0] > 1 else tables.shape[1]
-
-
-def _pools(kpool: torch.Tensor, vpool: torch.Tensor, n_kv_heads: int, head_dim: int) -> None:
-    for name, t in (("kpool", kpool), ("vpool", vpool)):
-        if not t.is_cuda or t.dtype not in _F16_BITS or t.dim() != 3 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous CUDA fp16 tensor [pages, page_size, kv_dim]")
-    if kpool.shape != vpool.shape or kpool.device != vpool.device:
-        raise ValueError("kpool and vpool must have the same shape and device")
-    if kpool.shape[2] < n_kv_heads * head_dim:
+def _pool_shape(kpool: torch.Tensor, vpool: torch.Tensor, dev: int, row: int) -> tuple:
+    """(pages, page size, kv_dim) of a layer's pools."""
+    shape = kpool.shape
+    if (len(shape) != 3 or vpool.shape != shape or kpool.dtype not in _F16_BITS or vpool.dtype not in _F16_BITS
+            or kpool.get_device() != dev or vpool.get_device() != dev or not kpool.is_contiguous()
+            or not vpool.is_contiguous()):
+        raise ValueError(f"kpool and vpool must be contiguous fp16 [pages, page_size, kv_dim] tensors of one shape on cuda:{dev}")
+    if shape[2] < row:
         raise ValueError("the pools' rows are shorter than n_kv_heads * head_dim")
+    return shape
 
 
-def _tokens(t: torch.Tensor, name: str, like: torch.Tensor, cols: int) -> None:
-    if (t.dim() != 2 or t.dtype != like.dtype or t.device != like.device or t.shape[0] != like.shape[0]
-            or t.shape[1] != cols or t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < cols)):
-        raise ValueError(f"{name} must be [{like.shape[0]}, {cols}] {like.dtype} on {like.device}, heads contiguous")
+def _token_stride(t: torch.Tensor, name: str, rows: int, cols: int, dtype: torch.dtype, dev: int) -> int:
+    """Elements between the tokens of a [rows, cols] activation tensor whose heads are contiguous."""
+    if t.dtype is dtype and t.get_device() == dev and t.dim() == 2:
+        n, m = t.shape
+        stride, one = t.stride()
+        if rows == 1:
+            stride = cols
+        if n == rows and m == cols and one == 1 and (stride >= cols or n == 0):
+            return stride
+    raise ValueError(f"{name} must be [{rows}, {cols}] {dtype} on cuda:{dev}, heads contiguous")
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _act_of(q: torch.Tensor) -> tuple:
+    """(YATTN_ACT_*, dtype, device index, rows) of the queries."""
+    act = _ACT.get(q.dtype)
+    dev = q.get_device()
+    if act is None or dev < 0 or q.dim() != 2:
+        raise ValueError("q must be a CUDA [tokens, heads*head_dim] tensor of float32, float16 or bfloat16")
+    return act, q.dtype, dev, q.shape[0]
 
 
 def page_step(kv_len_out: torch.Tensor, cu_new: torch.Tensor, slots: torch.Tensor, positions: torch.Tensor,
@@ -463,20 +492,20 @@ def page_step(kv_len_out: torch.Tensor, cu_new: torch.Tensor, slots: torch.Tenso
     """One serving step's block tables (tables and the free-page queue ring updated in place), slots and positions
     of the new tokens (slots.numel() is the token capacity), prefix sums and lengths, from kv_len and new_len (-1:
     the request ended).  state_out = {head, count, verdict, tokens}; see yattn_page_step for the verdicts."""
-    if not kv_len.is_cuda:
+    dev = kv_len.get_device()
+    if dev < 0:
         raise ValueError("kv_len must be a CUDA tensor")
-    _i32_on(kv_len, kv_len_out=kv_len_out, cu_new=cu_new, slots=slots, positions=positions, state_out=state_out,
-            ring=ring, state=state, kv_len=kv_len, new_len=new_len)
-    _tables(tables, kv_len)
-    n = kv_len.numel()
-    if new_len.numel() != n or kv_len_out.numel() != n or cu_new.numel() != n + 1 or tables.shape[0] != n:
-        raise ValueError("new_len, kv_len_out, cu_new (one more) and tables must have one entry per request of kv_len")
-    if positions.numel() != slots.numel() or state.numel() < 2 or state_out.numel() < 4:
+    _i32_on(dev, "kv_len new_len kv_len_out cu_new slots positions state_out ring state", kv_len, new_len, kv_len_out,
+            cu_new, slots, positions, state_out, ring, state)
+    n, cap = kv_len.numel(), slots.numel()
+    width, stride = _table_shape(tables, dev, n)
+    if new_len.numel() != n or kv_len_out.numel() != n or cu_new.numel() != n + 1:
+        raise ValueError("new_len, kv_len_out and cu_new (one more) must have one entry per request of kv_len")
+    if positions.numel() != cap or state.numel() < 2 or state_out.numel() < 4:
         raise ValueError("positions must match slots; state holds 2 values or more, state_out 4")
-    _call_on("yattn_page_step", kv_len, stream, kv_len_out.data_ptr(), cu_new.data_ptr(), slots.data_ptr(),
-             positions.data_ptr(), slots.numel(), state_out.data_ptr(), tables.data_ptr(), tables.shape[1],
-             _table_stride(tables), ring.data_ptr(), ring.numel(), state.data_ptr(), kv_len.data_ptr(),
-             new_len.data_ptr(), n, page_size)
+    _call_on("yattn_page_step", dev, stream, kv_len_out.data_ptr(), cu_new.data_ptr(), slots.data_ptr(),
+             positions.data_ptr(), cap, state_out.data_ptr(), tables.data_ptr(), width, stride, ring.data_ptr(),
+             ring.numel(), state.data_ptr(), kv_len.data_ptr(), new_len.data_ptr(), n, page_size)
 
 
 def rope_store_kv_paged(q_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kpool: torch.Tensor,
@@ -486,22 +515,19 @@ def rope_store_kv_paged(q_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
     """QK-norm (norm = qk_norm(...)), RoPE and the store of k and v into pages: q, k, v [tokens, heads*head_dim]
     (fp32, fp16 or bf16, any row stride), slots and positions from page_step; tokens with slot -1 are skipped.
     q_out may be q."""
-    if not q.is_cuda or q.dtype not in _ACT:
-        raise ValueError("q must be a CUDA tensor of float32, float16 or bfloat16")
-    for name, t, cols in (("q", q, n_heads * head_dim), ("q_out", q_out, n_heads * head_dim),
-                          ("k", k, n_kv_heads * head_dim), ("v", v, n_kv_heads * head_dim)):
-        _tokens(t, name, q, cols)
-    _pools(kpool, vpool, n_kv_heads, head_dim)
-    if kpool.device != q.device:
-        raise ValueError("the pools must be on q's device")
-    _i32_on(q, slots=slots, positions=positions)
-    if slots.numel() != q.shape[0] or positions.numel() != q.shape[0]:
+    act, dtype, dev, rows = _act_of(q)
+    cols, kv_cols = n_heads * head_dim, n_kv_heads * head_dim
+    pages, page_size, kv_dim = _pool_shape(kpool, vpool, dev, kv_cols)
+    _i32_on(dev, "slots positions", slots, positions)
+    if slots.numel() != rows or positions.numel() != rows:
         raise ValueError("slots and positions must have one entry per row of q")
-    _call_on("yattn_rope_store_kv_paged", q, stream, q_out.data_ptr(), _row_stride(q_out), q.data_ptr(),
-             _row_stride(q), k.data_ptr(), _row_stride(k), v.data_ptr(), _row_stride(v), _ACT[q.dtype],
-             kpool.data_ptr(), vpool.data_ptr(), kpool.shape[0] * kpool.shape[1], slots.data_ptr(),
-             positions.data_ptr(), q.shape[0], n_heads, n_kv_heads, head_dim, kpool.shape[2], rope_kind, n_rope_dims,
-             theta, _norm_arg(norm))
+    _call_on("yattn_rope_store_kv_paged", dev, stream, q_out.data_ptr(),
+             _token_stride(q_out, "q_out", rows, cols, dtype, dev), q.data_ptr(),
+             _token_stride(q, "q", rows, cols, dtype, dev), k.data_ptr(),
+             _token_stride(k, "k", rows, kv_cols, dtype, dev), v.data_ptr(),
+             _token_stride(v, "v", rows, kv_cols, dtype, dev), act, kpool.data_ptr(), vpool.data_ptr(),
+             pages * page_size, slots.data_ptr(), positions.data_ptr(), rows, n_heads, n_kv_heads, head_dim, kv_dim,
+             rope_kind, n_rope_dims, theta, _norm_arg(norm))
 
 
 _paged_ws: dict = {}   # (device, stream, head_dim) -> workspace of attn_paged's eager calls on that stream
@@ -515,14 +541,19 @@ def paged_workspace(head_dim: int, device=None) -> torch.Tensor:
 def _paged_workspace(head_dim: int, dev: int, stream) -> torch.Tensor:
     """The stream's own workspace: calls on one stream run in order, so they can share it.  A call being captured
     gets a fresh one (its zeroing is captured too): the graph may be replayed beside other work."""
-    with torch.cuda.device(dev), torch.cuda.stream(stream):
-        if torch.cuda.is_current_stream_capturing():
-            return paged_workspace(head_dim, torch.device("cuda", dev))
-        key = (dev, stream.cuda_stream, head_dim)
-        ws = _paged_ws.get(key)
-        if ws is None:
-            ws = _paged_ws[key] = paged_workspace(head_dim, torch.device("cuda", dev))
-        return ws
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return _paged_workspace(head_dim, dev, None)
+    if torch.cuda.current_device() != dev:
+        with torch.cuda.device(dev):
+            return _paged_workspace(head_dim, dev, None)
+    if torch.cuda.is_current_stream_capturing():
+        return paged_workspace(head_dim, torch.device("cuda", dev))
+    key = (dev, _raw_stream(dev), head_dim)
+    ws = _paged_ws.get(key)
+    if ws is None:
+        ws = _paged_ws[key] = paged_workspace(head_dim, torch.device("cuda", dev))
+    return ws
 
 
 def attn_paged(out: torch.Tensor, q: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, tables: torch.Tensor,
@@ -531,31 +562,24 @@ def attn_paged(out: torch.Tensor, q: torch.Tensor, kpool: torch.Tensor, vpool: t
     """Causal attention of ragged new tokens (rows cu_new[r]..cu_new[r+1] of q, fp32 / fp16 / bf16) over the first
     kv_len[r] rows of each request's pages, the new tokens' rows included; max_new bounds a request's new tokens.
     Rows of out behind the last request stay as they are."""
-    if not q.is_cuda or q.dtype not in _ACT:
-        raise ValueError("q must be a CUDA tensor of float32, float16 or bfloat16")
+    act, dtype, dev, rows = _act_of(q)
     cols = n_heads * head_dim
-    _tokens(q, "q", q, cols)
-    _tokens(out, "out", q, cols)
-    if gate is not None:
-        _tokens(gate, "gate", q, cols)
-    _pools(kpool, vpool, n_kv_heads, head_dim)
-    if kpool.device != q.device:
-        raise ValueError("the pools must be on q's device")
-    _i32_on(q, cu_new=cu_new, kv_len=kv_len)
-    _tables(tables, q)
+    pages, page_size, kv_dim = _pool_shape(kpool, vpool, dev, n_kv_heads * head_dim)
+    _i32_on(dev, "cu_new kv_len", cu_new, kv_len)
     n = kv_len.numel()
-    if cu_new.numel() != n + 1 or tables.shape[0] != n:
-        raise ValueError("cu_new (one more) and tables must have one entry per request of kv_len")
+    width, stride = _table_shape(tables, dev, n)
+    if cu_new.numel() != n + 1:
+        raise ValueError("cu_new must have one entry more than kv_len")
     if workspace is None:
-        dev = q.device.index
-        workspace = _paged_workspace(head_dim, dev, stream if stream is not None else torch.cuda.current_stream(dev))
-    elif workspace.device != q.device or not workspace.is_contiguous():
-        raise ValueError("workspace must be a contiguous tensor on q's device (paged_workspace)")
-    _call_on("yattn_attn_paged", q, stream, out.data_ptr(), _row_stride(out), q.data_ptr(), _row_stride(q),
-             _ptr(gate), _row_stride(gate) if gate is not None else 0, _ACT[q.dtype], kpool.data_ptr(),
-             vpool.data_ptr(), kpool.shape[0], kpool.shape[1], tables.data_ptr(), tables.shape[1],
-             _table_stride(tables), cu_new.data_ptr(), kv_len.data_ptr(), n, q.shape[0], max_new, n_heads, n_kv_heads,
-             head_dim, kpool.shape[2], workspace.data_ptr(), workspace.numel() * workspace.element_size())
+        workspace = _paged_workspace(head_dim, dev, stream)
+    elif workspace.get_device() != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on cuda:{dev} (paged_workspace)")
+    _call_on("yattn_attn_paged", dev, stream, out.data_ptr(), _token_stride(out, "out", rows, cols, dtype, dev),
+             q.data_ptr(), _token_stride(q, "q", rows, cols, dtype, dev), None if gate is None else gate.data_ptr(),
+             0 if gate is None else _token_stride(gate, "gate", rows, cols, dtype, dev), act, kpool.data_ptr(),
+             vpool.data_ptr(), pages, page_size, tables.data_ptr(), width, stride, cu_new.data_ptr(),
+             kv_len.data_ptr(), n, rows, max_new, n_heads, n_kv_heads, head_dim, kv_dim, workspace.data_ptr(),
+             workspace.nbytes)
 
 
 def sess_kv_save(kv: torch.Tensor, n_blocks: int, kv_dim: int, max_seq: int, pos: int, path: str,

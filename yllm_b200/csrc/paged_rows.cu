@@ -287,18 +287,21 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                 }
 #pragma unroll
                 for (int mt = 0; mt < KS; ++mt) {
-                    oc[mt][0] *= al_a;
-                    oc[mt][1] *= al_b;
-                    oc[mt][2] *= al_a;
-                    oc[mt][3] *= al_b;
                     uint32_t a[4];
                     ldsm_x4_t(v_addr(vt, mt), a);
                     a[0] &= vm01;
                     a[1] &= vm01;
                     a[2] &= vm23;
                     a[3] &= vm23;
-                    mma16816(oc[mt], a, ph0, ph1);
-                    mma16816(oc[mt], a, pl0, pl1);
+                    // a sum of its own, added in fp32: the tensor core truncates where it adds to an accumulator,
+                    // and over a long context those half ulps all point towards zero
+                    float d[4] = {};
+                    mma16816(d, a, pl0, pl1);
+                    mma16816(d, a, ph0, ph1);
+                    oc[mt][0] = fmaf(oc[mt][0], al_a, d[0]);
+                    oc[mt][1] = fmaf(oc[mt][1], al_b, d[1]);
+                    oc[mt][2] = fmaf(oc[mt][2], al_a, d[2]);
+                    oc[mt][3] = fmaf(oc[mt][3], al_b, d[3]);
                 }
                 __syncwarp();   // P^T is rewritten by the next step
             }

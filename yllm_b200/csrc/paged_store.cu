@@ -9,12 +9,18 @@
 // an ulp of the angle); here it is a product in 64 bits, reduced to a half turn before it is rounded, so
 // every angle is good to 1 ulp of its sine and cosine however far the position.
 //
-// One CTA per token.  A thread holds two VEC-element chunks of one head, VEC * size = 16 bytes, placed so
-// that both elements of each of its pairs are its own (half-split pairs: chunk c and chunk c + n/2;
-// neighbour pairs and unrotated dims: two chunks in a row).  So a head is hd / (2 VEC) consecutive lanes
-// (4 to 32), its sum of squares is a shuffle reduction among them, and every global access is a 16-byte
-// vector (8 for the fp16 rows of fp32 activations).  The token's sines and cosines, n/2 pairs shared by
-// all its heads, are computed once by the first threads while the row's loads are in flight.
+// A thread holds two VEC-element chunks of one head, VEC * size = 16 bytes, placed so that both elements
+// of each of its pairs are its own (half-split pairs: chunk c and chunk c + n/2; neighbour pairs and
+// unrotated dims: two chunks in a row).  So a head is hd / (2 VEC) consecutive lanes (4 to 32), its sum of
+// squares is a shuffle reduction among them, and every global access is a 16-byte vector (8 for the fp16
+// rows of fp32 activations).
+//
+// A CTA covers a token's heads (or a slice of them, where they pass 512 threads) and walks over tokens
+// with the next token's loads in flight, so the chain of one token -- load, norm, rotate, store -- hides
+// behind the others.  Sines and cosines, shared by a token's heads, go through shared memory, two buffers
+// in turn and four tokens at a time: with one barrier per token the barrier was the kernel's largest stall
+// (the fp64 angle and sincospif of one warp behind it; 16384 tokens of the qwen3.5 shape took 161 us).
+// The norm weights are read from global memory once per CTA.
 //
 // Bound: HBM.  q, k and v are read once, q_out and the cache rows written once.
 #include "common.cuh"
@@ -44,23 +50,22 @@ struct StoreParams {
     float eps;
     uint64_t q_stride, k_stride, v_stride, qo_stride;   // elements between tokens
     uint64_t n_rows;                 // rows of each pool
-    uint32_t n_heads, n_kv, kv_dim;
+    uint32_t n_tokens, n_heads, n_kv, kv_dim;
+    uint32_t group;                  // tokens per barrier
     uint32_t neighbour;              // pairs (2j, 2j+1); else (j, j + n_dims/2)
     uint32_t n_dims;
     int* status;
     double half_turns[kMaxPairs];    // theta^(-2j/n_dims) / pi: half turns per position
 };
 
-// VEC consecutive activations as fp32 (16 bytes read), and back (rounded to nearest).
-__device__ __forceinline__ void load_vec(const float* p, float (&x)[4]) {
-    const float4 v = __ldcs(reinterpret_cast<const float4*>(p));
-    x[0] = v.x;
-    x[1] = v.y;
-    x[2] = v.z;
-    x[3] = v.w;
+// 16 bytes of activations as fp32, and back (rounded to nearest).
+__device__ __forceinline__ void widen(const uint4& v, const float*, float (&x)[4]) {
+    x[0] = __uint_as_float(v.x);
+    x[1] = __uint_as_float(v.y);
+    x[2] = __uint_as_float(v.z);
+    x[3] = __uint_as_float(v.w);
 }
-__device__ __forceinline__ void load_vec(const __half* p, float (&x)[8]) {
-    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
+__device__ __forceinline__ void widen(const uint4& v, const __half*, float (&x)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -69,8 +74,7 @@ __device__ __forceinline__ void load_vec(const __half* p, float (&x)[8]) {
         x[2 * i + 1] = f.y;
     }
 }
-__device__ __forceinline__ void load_vec(const __nv_bfloat16* p, float (&x)[8]) {
-    const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p));
+__device__ __forceinline__ void widen(const uint4& v, const __nv_bfloat16*, float (&x)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -99,139 +103,197 @@ __device__ __forceinline__ void store_vec(__nv_bfloat16* p, const float (&x)[8])
     }
     *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
-// Cache rows: the engine's rounding, as every other store into the cache.
+// Cache rows: the engine's rounding, as every other store into the cache.  From 2^-14 up it adds half a
+// step to the magnitude and truncates, which leaves an fp16 value; smaller ones and NaN take the long form.
+__device__ __forceinline__ uint32_t cache_bits(float x) {
+    const uint32_t b = __float_as_uint(x);
+    if ((b & 0x7fffffffu) - 0x38800000u <= 0x7f800000u - 0x38800000u)
+        return __half_as_ushort(__float2half_rn(__uint_as_float((b + 0x1000u) & 0xffffe000u)));
+    return engine_f32_to_f16(x);
+}
 template <int VEC> __device__ __forceinline__ void store_cache(uint16_t* p, const float (&x)[VEC]) {
     uint32_t w[VEC / 2];
 #pragma unroll
-    for (int i = 0; i < VEC / 2; ++i)
-        w[i] = engine_f32_to_f16(x[2 * i]) | static_cast<uint32_t>(engine_f32_to_f16(x[2 * i + 1])) << 16;
+    for (int i = 0; i < VEC / 2; ++i) w[i] = cache_bits(x[2 * i]) | cache_bits(x[2 * i + 1]) << 16;
     if constexpr (VEC == 4)
         *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     else
         *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__device__ __forceinline__ float norm_w(const StoreParams& p, const void* w, uint32_t e) {
-    return p.norm_f16 ? h2f(static_cast<const uint16_t*>(w)[e]) : static_cast<const float*>(w)[e];
+// N floats from 16-byte aligned shared memory.
+template <int N> __device__ __forceinline__ void lds(const float* p, float (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p + i);
+        x[i] = v.x;
+        x[i + 1] = v.y;
+        x[i + 2] = v.z;
+        x[i + 3] = v.w;
+    }
 }
+
+constexpr uint32_t kGroup = 4;   // tokens per barrier, where there are more tokens than CTAs
 
 template <typename T, int HD>
 __global__ void __launch_bounds__(512) k_paged_store(const __grid_constant__ StoreParams p) {
     constexpr int VEC = 16 / sizeof(T);
     constexpr uint32_t LPH = HD / (2 * VEC);          // lanes per head
     static_assert(LPH <= 32 && (LPH & (LPH - 1)) == 0, "a head lies in one warp");
-    __shared__ float2 s_cs[kMaxPairs];
-    const size_t t = blockIdx.x;
-    const int32_t slot = p.slots[t];
-    if (slot < 0) return;                             // a padded token: nothing is read or written
+    __shared__ __align__(16) float s_cos[2][kGroup][kMaxPairs], s_sin[2][kGroup][kMaxPairs];
+    __shared__ __align__(16) float s_w[2][HD];        // QK-norm weights of q and k heads
     const uint32_t half = p.n_dims / 2;
-    const uint32_t n_items = (p.n_heads + 2 * p.n_kv) * LPH;
-    bool ready = false;
-    for (uint32_t base = 0; base < n_items; base += blockDim.x) {
-        const uint32_t item = base + threadIdx.x;
-        const uint32_t head = item / LPH, u = item % LPH;   // q heads, k heads, v heads
-        const bool live = item < n_items;
-        const bool is_q = head < p.n_heads, is_v = head >= p.n_heads + p.n_kv;
-        const uint32_t h = is_q ? head : is_v ? head - p.n_heads - p.n_kv : head - p.n_heads;
-        // this thread's two chunks of the head
-        uint32_t ea = u * 2 * VEC, eb = ea + VEC;
-        const bool split = !p.neighbour && !is_v && u * VEC < half;
-        if (split) {
-            ea = u * VEC;
-            eb = ea + half;
-        }
-        float a[VEC], b[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) a[i] = b[i] = 0.f;
+    // this thread's item: two chunks of a q, k or v head, the same for every token
+    const uint32_t item = blockIdx.y * blockDim.x + threadIdx.x;
+    const uint32_t head = item / LPH, u = item % LPH;
+    const bool live = head < p.n_heads + 2 * p.n_kv;
+    const bool is_q = head < p.n_heads, is_v = head >= p.n_heads + p.n_kv;
+    const uint32_t h = is_q ? head : is_v ? head - p.n_heads - p.n_kv : head - p.n_heads;
+    const bool split = !p.neighbour && !is_v && u * VEC < half;
+    const uint32_t ea = split ? u * VEC : u * 2 * VEC;
+    const uint32_t eb = split ? ea + half : ea + VEC;
+    const T* src = static_cast<const T*>(is_q ? p.q : is_v ? p.v : p.k) + h * HD;
+    const uint64_t src_stride = is_q ? p.q_stride : is_v ? p.v_stride : p.k_stride;
+    uint16_t* pool = (is_v ? p.vpool : p.kpool) + h * HD;
+    auto fetch = [&](size_t t, uint4& ra, uint4& rb) {
         if (live) {
-            const T* src = is_q ? static_cast<const T*>(p.q) + t * p.q_stride
-                                : is_v ? static_cast<const T*>(p.v) + t * p.v_stride
-                                       : static_cast<const T*>(p.k) + t * p.k_stride;
-            load_vec(src + h * HD + ea, a);
-            load_vec(src + h * HD + eb, b);
+            const T* row = src + t * src_stride;
+            ra = __ldcs(reinterpret_cast<const uint4*>(row + ea));
+            rb = __ldcs(reinterpret_cast<const uint4*>(row + eb));
         }
-        if (!ready) {                                 // while those loads are in flight
-            const double pos = static_cast<double>(p.positions[t]);
-            for (uint32_t j = threadIdx.x; j < half; j += blockDim.x) {
-                double ht = pos * p.half_turns[j];
-                ht -= 2.0 * rint(0.5 * ht);           // [-1, 1] half turns
-                float s, c;
-                sincospif(static_cast<float>(ht), &s, &c);
-                s_cs[j] = make_float2(c, s);
-            }
-            __syncthreads();
-            ready = true;
-        }
+    };
+
+    auto process = [&](size_t t, int32_t slot, const uint4& ra, const uint4& rb, const float* cs, const float* sn) {
+        float a[VEC], b[VEC];
+        widen(ra, static_cast<const T*>(nullptr), a);
+        widen(rb, static_cast<const T*>(nullptr), b);
         if (p.q_w) {                                  // every lane of the warp takes part
             float ss = 0.f;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) ss += a[i] * a[i] + b[i] * b[i];
 #pragma unroll
             for (uint32_t o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if (live && !is_v) {
-                const float inv = 1.0f / sqrtf(ss * (1.0f / HD) + p.eps);
-                const void* w = is_q ? p.q_w : p.k_w;
+            if (!is_v) {
+                const float m = ss * (1.0f / HD) + p.eps;
+                float inv = rsqrtf(m);
+                inv = inv * (1.5f - 0.5f * m * inv * inv);   // one Newton step: rsqrt.approx is 2 ulp off
+                float wa[VEC], wb[VEC];
+                lds(s_w[is_q ? 0 : 1] + ea, wa);
+                lds(s_w[is_q ? 0 : 1] + eb, wb);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    a[i] = a[i] * norm_w(p, w, ea + i) * inv;
-                    b[i] = b[i] * norm_w(p, w, eb + i) * inv;
+                    a[i] = a[i] * wa[i] * inv;
+                    b[i] = b[i] * wb[i] * inv;
                 }
             }
         }
-        if (!live) continue;
-        if (!is_v) {
-            if (split) {
+        if (split) {
+            float c[VEC], s[VEC];
+            lds(cs + ea, c);
+            lds(sn + ea, s);
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const float2 cs = s_cs[ea + i];
-                    const float x = a[i], y = b[i];
-                    a[i] = x * cs.x - y * cs.y;
-                    b[i] = x * cs.y + y * cs.x;
-                }
-            } else if (p.neighbour) {
+            for (int i = 0; i < VEC; ++i) {
+                const float x = a[i], y = b[i];
+                a[i] = x * c[i] - y * s[i];
+                b[i] = x * s[i] + y * c[i];
+            }
+        } else if (p.neighbour && !is_v) {            // pairs ea/2 .. ea/2 + VEC - 1: chunk a's, then chunk b's
+            float c[VEC], s[VEC];
+            lds(cs + ea / 2, c);
+            lds(sn + ea / 2, s);
 #pragma unroll
-                for (int i = 0; i < VEC; i += 2) {
-                    const float2 ca = s_cs[(ea + i) / 2], cb = s_cs[(eb + i) / 2];
-                    const float xa = a[i], ya = a[i + 1], xb = b[i], yb = b[i + 1];
-                    a[i] = xa * ca.x - ya * ca.y;
-                    a[i + 1] = xa * ca.y + ya * ca.x;
-                    b[i] = xb * cb.x - yb * cb.y;
-                    b[i + 1] = xb * cb.y + yb * cb.x;
-                }
+            for (int i = 0; i < VEC / 2; ++i) {
+                const float xa = a[2 * i], ya = a[2 * i + 1], xb = b[2 * i], yb = b[2 * i + 1];
+                a[2 * i] = xa * c[i] - ya * s[i];
+                a[2 * i + 1] = xa * s[i] + ya * c[i];
+                b[2 * i] = xb * c[VEC / 2 + i] - yb * s[VEC / 2 + i];
+                b[2 * i + 1] = xb * s[VEC / 2 + i] + yb * c[VEC / 2 + i];
             }
         }
-        if (is_q) {
+        if (!live) {
+        } else if (is_q) {
             T* dst = static_cast<T*>(p.q_out) + t * p.qo_stride + h * HD;
             store_vec(dst + ea, a);
             store_vec(dst + eb, b);
         } else if (static_cast<uint64_t>(slot) < p.n_rows) {
-            uint16_t* dst = (is_v ? p.vpool : p.kpool) + static_cast<size_t>(slot) * p.kv_dim + h * HD;
+            uint16_t* dst = pool + static_cast<size_t>(slot) * p.kv_dim;
             store_cache<VEC>(dst + ea, a);
             store_cache<VEC>(dst + eb, b);
         } else if (u == 0) {
             atomicCAS(p.status, 0, ST_PAGED_BAD_PAGE);
         }
+    };
+
+    const size_t n = p.n_tokens, group = p.group;     // 1 or kGroup tokens per barrier
+    size_t t = blockIdx.x * group;                    // < n_tokens
+    uint4 ra = {}, rb = {};
+    fetch(t, ra, rb);
+    int32_t slot = p.slots[t];
+    if (p.q_w) {                                      // published by the first group's barrier
+        for (uint32_t i = threadIdx.x; i < 2 * HD; i += blockDim.x) {
+            const void* w = i < HD ? p.q_w : p.k_w;
+            const uint32_t e = i % HD;
+            s_w[i / HD][e] = p.norm_f16 ? h2f(static_cast<const uint16_t*>(w)[e]) : static_cast<const float*>(w)[e];
+        }
+    }
+    // this thread's first pair of a group, whose position is loaded a group ahead
+    const uint32_t j0 = threadIdx.x % half, k0 = threadIdx.x / half;
+    const double f0 = p.half_turns[j0];
+    int32_t pos0 = k0 < group && t + k0 < n ? p.positions[t + k0] : 0;
+    for (uint32_t buf = 0; t < n; buf ^= 1) {
+        const size_t t_next = t + gridDim.x * group;  // the next group
+        for (uint32_t i = threadIdx.x; i < group * half; i += blockDim.x) {
+            const bool first = i == threadIdx.x;
+            const uint32_t k = first ? k0 : i / half, j = first ? j0 : i % half;
+            if (t + k >= n) break;
+            double ht = first ? pos0 * f0 : p.positions[t + k] * p.half_turns[j];
+            ht -= 2.0 * rint(0.5 * ht);               // [-1, 1] half turns
+            sincospif(static_cast<float>(ht), &s_sin[buf][k][j], &s_cos[buf][k][j]);
+        }
+        pos0 = k0 < group && t_next + k0 < n ? p.positions[t_next + k0] : 0;
+        __syncthreads();
+        for (uint32_t k = 0; k < group && t < n; ++k) {
+            const size_t tn = k + 1 < group && t + 1 < n ? t + 1 : t_next;
+            uint4 na = {}, nb = {};
+            int32_t nslot = -1;
+            if (tn < n) {
+                fetch(tn, na, nb);
+                nslot = p.slots[tn];
+            }
+            if (slot >= 0) process(t, slot, ra, rb, s_cos[buf][k], s_sin[buf][k]);   // else a padded token
+            const bool last = tn == t_next;
+            t = tn;
+            ra = na;
+            rb = nb;
+            slot = nslot;
+            if (last) break;
+        }
     }
 }
 
 template <typename T, int HD>
-int launch_store(const StoreParams& p, uint32_t n_tokens, cudaStream_t st, char* err, size_t errlen) {
+int launch_store(const StoreParams& p, uint32_t sms, cudaStream_t st, char* err, size_t errlen) {
     constexpr uint32_t LPH = HD / (2 * (16 / sizeof(T)));
     const uint32_t items = (p.n_heads + 2 * p.n_kv) * LPH;
-    // one pass over the token's items where they fit a block of 512, else equal passes
-    const uint32_t passes = (items + 511) / 512;
-    const uint32_t threads = ((items + passes - 1) / passes + 31) / 32 * 32;
-    k_paged_store<T, HD><<<n_tokens, threads, 0, st>>>(p);
+    const uint32_t slices = (items + 511) / 512;
+    const uint32_t threads = ((items + slices - 1) / slices + 31) / 32 * 32;
+    // as many CTAs as the SMs hold at 64 registers a thread; each walks over every gridDim.x-th group of tokens
+    const uint32_t resident = std::max(1u, std::min(16u, 1024u / threads));
+    const uint32_t most = std::max(1u, sms * resident / slices);
+    StoreParams q = p;
+    q.group = p.n_tokens > most ? kGroup : 1;
+    const uint32_t ctas = std::min((p.n_tokens + q.group - 1) / q.group, most);
+    k_paged_store<T, HD><<<dim3(ctas, slices), threads, 0, st>>>(q);
     YATTN_CHECK_LAUNCH(err, errlen, "rope_store_kv_paged");
     return 0;
 }
 
 template <typename T>
-int dispatch_store(const StoreParams& p, uint32_t hd, uint32_t n_tokens, cudaStream_t st, char* err, size_t errlen) {
+int dispatch_store(const StoreParams& p, uint32_t hd, uint32_t sms, cudaStream_t st, char* err, size_t errlen) {
     switch (hd) {
-        case 64: return launch_store<T, 64>(p, n_tokens, st, err, errlen);
-        case 128: return launch_store<T, 128>(p, n_tokens, st, err, errlen);
-        default: return launch_store<T, 256>(p, n_tokens, st, err, errlen);
+        case 64: return launch_store<T, 64>(p, sms, st, err, errlen);
+        case 128: return launch_store<T, 128>(p, sms, st, err, errlen);
+        default: return launch_store<T, 256>(p, sms, st, err, errlen);
     }
 }
 
@@ -331,6 +393,7 @@ extern "C" int yattn_rope_store_kv_paged(void* q_out, uint32_t q_out_stride, con
     p.v_stride = v_stride;
     p.qo_stride = q_out_stride;
     p.n_rows = n_rows;
+    p.n_tokens = n_tokens;
     p.n_heads = n_heads;
     p.n_kv = n_kv_heads;
     p.kv_dim = kv_dim;
@@ -352,8 +415,8 @@ extern "C" int yattn_rope_store_kv_paged(void* q_out, uint32_t q_out_stride, con
     std::copy(freq.f, freq.f + n_dims / 2, p.half_turns);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (act) {
-        case YATTN_ACT_F32: return dispatch_store<float>(p, head_dim, n_tokens, st, err, errlen);
-        case YATTN_ACT_F16: return dispatch_store<__half>(p, head_dim, n_tokens, st, err, errlen);
-        default: return dispatch_store<__nv_bfloat16>(p, head_dim, n_tokens, st, err, errlen);
+        case YATTN_ACT_F32: return dispatch_store<float>(p, head_dim, static_cast<uint32_t>(ctx->num_sms), st, err, errlen);
+        case YATTN_ACT_F16: return dispatch_store<__half>(p, head_dim, static_cast<uint32_t>(ctx->num_sms), st, err, errlen);
+        default: return dispatch_store<__nv_bfloat16>(p, head_dim, static_cast<uint32_t>(ctx->num_sms), st, err, errlen);
     }
 }
