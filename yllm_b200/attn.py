@@ -534,8 +534,10 @@ _paged_ws: dict = {}   # (device, stream, head_dim) -> workspace of attn_paged's
 
 
 def paged_workspace(head_dim: int, device=None) -> torch.Tensor:
-    """A zeroed workspace for attn_paged, for callers that keep their own (one per stream or graph in flight)."""
-    return torch.zeros(lib.yattn_attn_paged_workspace_bytes(head_dim), dtype=torch.uint8, device=device or "cuda")
+    """A workspace for attn_paged (its counters zeroed), for callers that keep their own (one per stream or graph in flight)."""
+    ws = torch.empty(lib.yattn_attn_paged_workspace_bytes(head_dim), dtype=torch.uint8, device=device or "cuda")
+    ws[:4096].zero_()
+    return ws
 
 
 def _paged_workspace(head_dim: int, dev: int, stream) -> torch.Tensor:

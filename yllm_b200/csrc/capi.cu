@@ -86,6 +86,25 @@ int encode_kv_map(CUtensorMap* map, const void* base, uint32_t kv_dim, uint64_t 
     return 0;
 }
 
+int encode_page_map(CUtensorMap* map, const void* base, uint32_t kv_dim, uint64_t n_rows, uint32_t cols,
+                    uint32_t box_rows, uint32_t box_panels, char* err, size_t errlen) {
+    auto enc = get_encode(err, errlen);
+    if (!enc) return -1;
+    cuuint64_t dims[4] = {64, 8, cols / 64, n_rows / 8};
+    cuuint64_t strides[3] = {static_cast<cuuint64_t>(kv_dim) * 2, 128, static_cast<cuuint64_t>(kv_dim) * 16};
+    cuuint32_t box[4] = {64, 8, box_panels, box_rows / 8};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_err(err, errlen, "cuTensorMapEncodeTiled (pages) failed (%d): kv_dim %u, %llu rows, box %u x %u",
+                static_cast<int>(r), kv_dim, static_cast<unsigned long long>(n_rows), box_rows, box_panels);
+        return -1;
+    }
+    return 0;
+}
+
 int encode_f32_store_map(CUtensorMap* map, void* base, uint32_t cols, uint32_t stride_elems, uint64_t n_rows,
                          uint32_t box_rows, char* err, size_t errlen) {
     auto enc = get_encode(err, errlen);

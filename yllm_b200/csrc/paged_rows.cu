@@ -7,9 +7,10 @@
 // the products carry about 22 bits of fp32's 24 for any activation type.
 //
 // One persistent CTA per SM walks its equal share of the schedule (paged.cuh).  A producer warp fills a
-// ring of stages (K and V of 16 tokens per consumer warp) with tensor copies, one box of min(page, stage)
-// rows x 64 dims per lane: the lanes look the pages up in the block table one stage ahead, so the lookup's
-// latency is off the stream.  With a unit's first stage goes its descriptor.  Consumer warps own one kv
+// ring of stages (K and V of 16 tokens per consumer warp) with tensor copies, one per page and lane: the
+// lanes look the pages up in the block table one stage ahead, so the lookup's latency is off the stream.
+// A copy brings all the unit's dims of min(page, stage) rows (4-D maps); with a copy per 64 dims, 2 KB
+// at 16-row pages, the copies' rate was the bound (64 ragged Llama-3-8B sequences: 232 us against 207).  With a unit's first stage goes its descriptor.  Consumer warps own one kv
 // head and 16 tokens of each stage; the warps' (m, l, o) meet in the unit's last stage.
 //
 // Bound: HBM, K and V once.
@@ -87,11 +88,9 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
         const uint32_t page = 1u << p.page_shift;
         const uint32_t box = min(page, TOK);                  // rows of a copy
         const uint32_t per_block = TOK / box;                 // pages of a stage
-        // this lane's copies: page i_pg of the stage, panels and K/V by lane (at most 32 per stage at 16-row
-        // pages: TOK / 16 * NPAN * 2 = 32, 16 at head_dim 64)
-        const uint32_t n_box = per_block * NPAN * 2;
-        const uint32_t i_pg = lane / (NPAN * 2), i_pan = (lane >> 1) % NPAN, i_v = lane & 1;
-        const bool mine = static_cast<uint32_t>(lane) < n_box;
+        // this lane's copy: K (even) or V (odd) of page lane / 2 of the stage (8 pages at most)
+        const uint32_t i_pg = lane >> 1, i_v = lane & 1;
+        const bool mine = i_pg < per_block;
         uint32_t gi = 0;
         bool ok = true;
         PagedUnit u;
@@ -101,8 +100,8 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
         };
         while (ok && sched.next(u)) {
             const uint32_t nt = max(1u, u.kb1 - u.kb0);
-            const int32_t x = static_cast<int32_t>(u.g * HC * HD + i_pan * 64);
-            // row of this lane's box in block b, or -1 behind the request's last key
+            const int32_t pan0 = static_cast<int32_t>(u.g * NPAN);
+            // row of this lane's copy in block b, or -1 behind the request's last key
             auto row_of = [&](uint32_t b) -> int32_t {
                 const uint32_t key = b * TOK + i_pg * box;
                 if (!mine || key >= static_cast<uint32_t>(u.len)) return -1;
@@ -117,11 +116,11 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                 }
                 if (i == 0 && lane == 0) *unit_at(s) = u;     // published by the arrive on full[s]
                 const uint32_t n_copy = __popc(__ballot_sync(0xffffffffu, row >= 0));
-                if (lane == 0) mbar_arrive_expect_tx(&full[s], n_copy * box * 128);
+                if (lane == 0) mbar_arrive_expect_tx(&full[s], n_copy * box * (NPAN * 128));
                 __syncwarp();
                 if (row >= 0)
-                    tma_load_2d(smem + s * C::STAGE + i_v * TILEB + i_pan * (TOK * 128) + i_pg * (box * 128),
-                                i_v ? &vmap : &kmap, x, row, &full[s]);
+                    tma_load_4d(smem + s * C::STAGE + i_v * TILEB + i_pg * box * (NPAN * 128), i_v ? &vmap : &kmap, 0,
+                                0, pan0, row >> 3, &full[s]);
                 row = i + 1 < nt ? row_of(u.kb0 + i + 1) : -1;
             }
         }
@@ -150,12 +149,14 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
     const uint32_t p_off = (lane & 7) * 48 + ((lane >> 3) & 1) * 16;
     const uint32_t rk = 16 * sl + (lane & 15), rv = 16 * sl + (lane & 7) + ((lane >> 4) & 1) * 8;
     const uint32_t hpan = hl * (HD / 64);
-    auto k_addr = [&](uint32_t kt, int kk) -> uint32_t {      // K fragment, k-step kk (128-byte swizzled panels)
-        return kt + (hpan + (kk >> 2)) * TOK * 128 + rk * 128 +
+    // a tile is 1024-byte atoms (8 rows of a 64-dim panel, 16-byte chunk c of row r at c ^ (r & 7)), panels then
+    // 8-row groups
+    auto k_addr = [&](uint32_t kt, int kk) -> uint32_t {      // K fragment, k-step kk
+        return kt + ((rk >> 3) * NPAN + hpan + (kk >> 2)) * 1024 + (lane & 7) * 128 +
                ((static_cast<uint32_t>(((kk & 3) << 1) + (lane >> 4)) ^ (lane & 7)) << 4);
     };
     auto v_addr = [&](uint32_t vt, int mt) -> uint32_t {      // V^T fragment, m-tile mt
-        return vt + (hpan + (mt >> 2)) * TOK * 128 + rv * 128 +
+        return vt + ((rv >> 3) * NPAN + hpan + (mt >> 2)) * 1024 + (lane & 7) * 128 +
                ((static_cast<uint32_t>(((mt & 3) << 1) + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
     };
 
@@ -458,8 +459,9 @@ int paged_rows(const PagedParams& pp, const uint16_t* kpool, const uint16_t* vpo
     const uint32_t ncw = hd >= 256 ? 4 : 8, tok = 16 * ncw / p.hc;
     const uint32_t box = std::min(1u << p.page_shift, tok);
     CUtensorMap mk, mv;
-    if (encode_kv_map(&mk, kpool, kv_dim, n_rows, box, err, errlen) ||
-        encode_kv_map(&mv, vpool, kv_dim, n_rows, box, err, errlen))
+    const uint32_t panels = p.hc * hd / 64;
+    if (encode_page_map(&mk, kpool, kv_dim, n_rows, n_kv * hd, box, panels, err, errlen) ||
+        encode_page_map(&mv, vpool, kv_dim, n_rows, n_kv * hd, box, panels, err, errlen))
         return -1;
     const uint32_t ctas = std::min<uint32_t>(static_cast<uint32_t>(dev_num_sms()), kPagedMaxPieces);
     switch (hd) {

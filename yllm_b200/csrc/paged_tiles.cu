@@ -13,7 +13,7 @@
 //   0-7  softmax: row r of the tile (TMEM lane r) belongs to warps r/32 and r/32 + 4, which halve each
 //        block's columns.  They fetch Q (hi to shared memory, lo to TMEM), turn S into P in place, rescale
 //        O when m grows by more than 2^8, and write the unit's rows or partials.
-//   8, 10  K and V blocks by tensor copies into their rings, a box of min(page, BN) rows x 64 dims per lane.
+//   8, 10  K and V blocks by tensor copies into their rings, one copy per page and lane (4-D maps).
 //   9    MMA issue.  S runs up to NSB blocks ahead of the softmax.
 //   11   the schedule: units into a ring of four descriptors, so finding the next unit is off the others' path.
 // V rows behind the last key the tile sees hold whatever the page held: the PV product stops at the 16-key
@@ -165,14 +165,13 @@ __global__ void __launch_bounds__(kTThreads, 1)
         const uint32_t depth = is_v ? VST : KST;
         if (lane == 0) prefetch_tensormap(map);
         const uint32_t page = 1u << p.page_shift, box = min(page, static_cast<uint32_t>(BN));
-        const uint32_t i_pg = lane / NPAN, i_pan = lane % NPAN;   // this lane's box of a block (16 at most)
+        const uint32_t i_pg = lane;                               // this lane's page of a block (8 at most)
         const bool mine = i_pg < BN / box;
         uint32_t s = 0, ph = 0, issued = 0;                       // ring stage, its pass's parity, blocks in all
         bool ok = true;
         PagedUnit u;
         for (uint32_t ui = 0; ok && get_unit(ui, u); ++ui) {
             const uint32_t kend = static_cast<uint32_t>(unit_keys(u));
-            const int32_t x = static_cast<int32_t>(u.g * HD + i_pan * 64);
             auto row_of = [&](uint32_t b) -> int32_t {
                 const uint32_t key = b * BN + i_pg * box;
                 if (!mine || key >= kend) return -1;
@@ -186,10 +185,11 @@ __global__ void __launch_bounds__(kTThreads, 1)
                     break;
                 }
                 const uint32_t n_copy = __popc(__ballot_sync(0xffffffffu, row >= 0));
-                if (lane == 0) mbar_arrive_expect_tx(&full[s], n_copy * box * 128);
+                if (lane == 0) mbar_arrive_expect_tx(&full[s], n_copy * box * (HD * 2));
                 __syncwarp();
                 if (row >= 0)
-                    tma_load_2d(ring + s * C::KV_BYTES + i_pan * (BN * 128) + i_pg * (box * 128), map, x, row, &full[s]);
+                    tma_load_4d(ring + s * C::KV_BYTES + i_pg * box * (HD * 2), map, 0, 0, static_cast<int32_t>(u.g * NPAN),
+                                row >> 3, &full[s]);
                 ++issued;
                 if (++s == depth) {
                     s = 0;
@@ -209,8 +209,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
         constexpr uint32_t IDESC_PV = idesc_f16(BM, HD, 1);
         // an operand at base + off has the base's descriptor + off / 16
         const uint64_t dq0 = sdesc_sw128(sQ, 16, 1024);
-        const uint64_t dk0 = sdesc_sw128(sK, 16, 1024);
-        const uint64_t dv0 = sdesc_sw128(sV, BN * 128, 1024);
+        // K and V tiles: 1024-byte atoms of 8 rows x 64 dims, panels 1024 B and row groups NPAN * 1024 B apart
+        const uint64_t dk0 = sdesc_sw128(sK, 16, NPAN * 1024);
+        const uint64_t dv0 = sdesc_sw128(sV, 1024, NPAN * 1024);
         uint32_t ks = 0, kph = 0, vs = 0, vph = 0;      // ring stages and parities
         uint32_t s_sb = 0, pv_sb = 0, pv_ph = 0;        // S buffer of the next S product, of the next PV product
         uint32_t qph = 0;
@@ -237,13 +238,13 @@ __global__ void __launch_bounds__(kTThreads, 1)
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; ++kk) {
                         const uint64_t a = dq0 + (((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4);
-                        const uint64_t b = dk + (((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
+                        const uint64_t b = dk + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4);
                         umma_f16(d, a, b, IDESC_QK, kk > 0 ? 1u : 0u);
                     }
                     if constexpr (PREC) {   // + Q_lo K^T, A from TMEM
 #pragma unroll
                         for (int kk = 0; kk < HD / 16; ++kk) {
-                            const uint64_t b = dk + (((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
+                            const uint64_t b = dk + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4);
                             umma_f16_ts(d, tmem + C::qlo_col(kk), b, IDESC_QK, 1u);
                         }
                     }
@@ -270,7 +271,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                     const int zrows = steps * 16 - valid;
                     for (int i = lane; i < zrows * NPAN * 8; i += 32) {
                         const int row = valid + i / (NPAN * 8), c = i % (NPAN * 8);
-                        *reinterpret_cast<uint4*>(sV + vs * C::KV_BYTES + (c >> 3) * (BN * 128) + row * 128 + (c & 7) * 16) =
+                        *reinterpret_cast<uint4*>(sV + vs * C::KV_BYTES + ((row >> 3) * NPAN + (c >> 3)) * 1024 + (row & 7) * 128 + (c & 7) * 16) =
                             make_uint4(0u, 0u, 0u, 0u);
                     }
                     fence_proxy_async_smem();
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                         for (int kk = 0; kk < BN / 16; ++kk)
                             if (kk < steps)
                                 umma_f16_ts(tmem + C::COL_O, pcol + 32 * (kk >> 1) + 16 * plane + 8 * (kk & 1),
-                                            dv + ((kk * 16 * 128) >> 4), IDESC_PV,
+                                            dv + ((kk * 2 * NPAN * 1024) >> 4), IDESC_PV,
                                             (jj > 0 || plane > 0 || kk > 0) ? 1u : 0u);
                     umma_commit(&bars->v_empty[vs]);
                     umma_commit(&bars->pv_done[pv_sb]);
@@ -696,8 +697,8 @@ int paged_tiles(const PagedParams& pp, const uint16_t* kpool, const uint16_t* vp
     p.n_groups = n_kv;
     const uint32_t bn = hd >= 256 ? 64 : 128, box = std::min(1u << p.page_shift, bn);
     CUtensorMap mk, mv;
-    if (encode_kv_map(&mk, kpool, kv_dim, n_rows, box, err, errlen) ||
-        encode_kv_map(&mv, vpool, kv_dim, n_rows, box, err, errlen))
+    if (encode_page_map(&mk, kpool, kv_dim, n_rows, n_kv * hd, box, hd / 64, err, errlen) ||
+        encode_page_map(&mv, vpool, kv_dim, n_rows, n_kv * hd, box, hd / 64, err, errlen))
         return -1;
     const uint32_t ctas = std::min<uint32_t>(static_cast<uint32_t>(dev_num_sms()), kPagedMaxPieces);
     const bool prec = p.act == YATTN_ACT_F32;

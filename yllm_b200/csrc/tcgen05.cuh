@@ -11,6 +11,14 @@ namespace yattn {
 int encode_kv_map(CUtensorMap* map, const void* base, uint32_t kv_dim, uint64_t n_rows, uint32_t box_rows, char* err,
                   size_t errlen);
 
+// Host: 4-D view (64 elements, 8 rows, 64-element panels, 8-row groups) of fp16 rows of kv_dim elements, the
+// first `cols` of each (a multiple of 64), n_rows (a multiple of 8) rows; box 64 x 8 x box_panels x box_rows/8,
+// 128-byte swizzle.  One copy fetches box_rows rows of all its panels, laid out as 1024-byte atoms (8 rows of a
+// panel): panels 1024 B apart, 8-row groups box_panels * 1024 B apart, so copies of any number of row groups
+// stack into one matrix operand.
+int encode_page_map(CUtensorMap* map, const void* base, uint32_t kv_dim, uint64_t n_rows, uint32_t cols,
+                    uint32_t box_rows, uint32_t box_panels, char* err, size_t errlen);
+
 // Host: 2-D tensor map over fp32 rows of `cols` elements (row stride stride_elems*4 B,
 // a multiple of 16), n_rows rows from base; box 32 elements (128 B) x box_rows rows,
 // 128-byte swizzle.  Used for stores: rows and columns outside the map are not written.
@@ -27,6 +35,16 @@ __device__ __forceinline__ void tma_load_2d(void* dst_smem, const CUtensorMap* m
         "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
         "[%4];" ::"r"(smem_u32(dst_smem)),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// 4-D tiled load of one box (encode_page_map).
+__device__ __forceinline__ void tma_load_4d(void* dst_smem, const CUtensorMap* map, int32_t c0, int32_t c1, int32_t c2,
+                                            int32_t c3, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(smem_u32(dst_smem)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
         : "memory");
 }
 
