@@ -8,8 +8,8 @@
 // the pieces in piece order, so the result does not depend on who was last.  The shares are equal
 // whatever the lengths: one long context spreads over every SM, and 64 ragged ones fill them evenly.
 //
-// The line is never built: w summed over a request's tiles has a closed form, so a CTA needs one pass
-// over (cu, kv_len) -- a block-wide sum and scan -- and then walks its units in order.
+// The line is never built: w summed over a request's tiles has a closed form, so one warp of the CTA needs
+// one pass over (cu, kv_len) -- a sum and a scan -- and then walks its units in order.
 #pragma once
 
 #include "common.cuh"
@@ -48,15 +48,69 @@ __device__ __forceinline__ float2 ld_act2(const void* p, size_t i, int act) {
     if (act == YATTN_ACT_F16) return h2f2(w);
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
-__device__ __forceinline__ float ld_act(const void* p, size_t i, int act) {
-    if (act == YATTN_ACT_F32) return static_cast<const float*>(p)[i];
-    const uint16_t w = static_cast<const uint16_t*>(p)[i];
-    return act == YATTN_ACT_F16 ? h2f(w) : __uint_as_float(static_cast<uint32_t>(w) << 16);
+// N = 2, 4 or 8 consecutive values (N * size aligned): activations out, fp32 in shared or global memory.
+template <int N> __device__ __forceinline__ void st_act_vec(void* p, size_t i, int act, const float (&x)[N]) {
+    if (act == YATTN_ACT_F32) {
+        float* d = static_cast<float*>(p) + i;
+        if constexpr (N == 2) *reinterpret_cast<float2*>(d) = make_float2(x[0], x[1]);
+        else
+#pragma unroll
+            for (int k = 0; k < N; k += 4) *reinterpret_cast<float4*>(d + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+        return;
+    }
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int k = 0; k < N / 2; ++k) {
+        if (act == YATTN_ACT_F16) {
+            const __half2 h = __floats2half2_rn(x[2 * k], x[2 * k + 1]);
+            w[k] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * k], x[2 * k + 1]);
+            w[k] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+    }
+    uint16_t* d = static_cast<uint16_t*>(p) + i;
+    if constexpr (N == 2) *reinterpret_cast<uint32_t*>(d) = w[0];
+    else if constexpr (N == 4) *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
 }
-__device__ __forceinline__ void st_act(void* p, size_t i, int act, float x) {
-    if (act == YATTN_ACT_F32) static_cast<float*>(p)[i] = x;
-    else if (act == YATTN_ACT_F16) static_cast<__half*>(p)[i] = __float2half_rn(x);
-    else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+template <int N> __device__ __forceinline__ void ld_vec(const float* p, float (&x)[N]) {
+    if constexpr (N == 2) {
+        const float2 v = *reinterpret_cast<const float2*>(p);
+        x[0] = v.x;
+        x[1] = v.y;
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + k);
+            x[k] = v.x;
+            x[k + 1] = v.y;
+            x[k + 2] = v.z;
+            x[k + 3] = v.w;
+        }
+    }
+}
+template <int N> __device__ __forceinline__ void ldcg_vec_n(const float* p, float (&x)[N]) {
+    if constexpr (N == 2) {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(p));
+        x[0] = v.x;
+        x[1] = v.y;
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; k += 4) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(p + k));
+            x[k] = v.x;
+            x[k + 1] = v.y;
+            x[k + 2] = v.z;
+            x[k + 3] = v.w;
+        }
+    }
+}
+template <int N> __device__ __forceinline__ void st_vec(float* p, const float (&x)[N]) {
+    if constexpr (N == 2) *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
+    else
+#pragma unroll
+        for (int k = 0; k < N; k += 4) *reinterpret_cast<float4*>(p + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
 }
 __device__ __forceinline__ float sigmoid_of(float x) { return 1.0f / (1.0f + __expf(-x)); }
 
@@ -113,18 +167,27 @@ struct PagedUnit {
     uint32_t done;              // 1: no unit, the list has ended
 };
 
+// a / b; the usual operands fit 32 bits, where the division is several times shorter.
+__device__ __forceinline__ long long div_pos(long long a, long long b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+
 // ROWS: query rows per tile (a row is one token x one head of the group); 0: a request's rows are one tile.
+// One warp runs it, all lanes.
 template <int BN, int ROWS> struct PagedSched {
-    // keys charged for a unit besides its own, shortest share, and least blocks at a cut
+    // Keys charged for a unit besides its own, and the least keys of a share where units are cut.  A cut costs a
+    // partial's round trip through memory, about 2.5 us, and a block of the decode form 0.9 us when nothing else
+    // runs: shares of 128 beat 512 there from 512 keys on (one Llama-3-8B sequence, 1024 keys: 12.0 us against
+    // 17.6), and cutting a unit less than about fourfold loses (256 keys: 12.0 us cut, 11.1 whole).
     static constexpr long long kUnitCost = ROWS ? 384 : 192;
-    static constexpr long long kMinShare = ROWS ? 512 : 256;
-    static constexpr uint32_t kSnap = 1;
-    // a share inside a unit holds a block: a unit charges at most BN + 128 keys per block once it has two
-    static_assert(kMinShare >= BN + 128 && kUnitCost / kMinShare < 8, "pieces are contiguous and found in one probe");
+    static constexpr long long kMinShare = ROWS ? 256 : 128;
+    static_assert(kUnitCost >= BN && kMinShare >= BN, "a share inside a unit holds a block, so a cut unit's pieces are contiguous CTAs");
 
     const PagedParams& p;
     int lane;
     long long W, total, x0, x1;   // weight of a head group and in all; this CTA's share
+    long long per, rem;           // total = per * n_active + rem: the first rem shares are one longer
     long long base;               // weight of the group's requests before r
     uint32_t n_active, cta, g, r, j;
 
@@ -134,110 +197,112 @@ template <int BN, int ROWS> struct PagedSched {
         if (!ROWS) return q.n > 0 ? 1u : 0u;
         return (static_cast<uint32_t>(q.n) * p.group + ROWS - 1) / (ROWS ? ROWS : 1);
     }
-    // weight of the request's tiles before tile t
+    // weight of the request's tiles before tile t: kUnitCost and about the keys its last row sees, each
     static __device__ __forceinline__ long long before(const PagedParams& p, const PagedReq& q, uint32_t t) {
         if (!ROWS) return t ? kUnitCost + q.len : 0;
         const long long T = t;
-        return T * (kUnitCost + max(q.len - q.n, 0)) + T * (T + 1) * (ROWS / 2) / p.group;
+        return T * (kUnitCost + max(q.len - q.n, 0)) + div_pos(T * (T + 1) * (ROWS / 2), p.group);
     }
     static __device__ __forceinline__ long long weight(const PagedParams& p, const PagedReq& q) {
         return before(p, q, tiles(p, q));
     }
-    // key blocks of tile t: up to the last position its rows see
-    static __device__ __forceinline__ uint32_t blocks(const PagedParams& p, const PagedReq& q, uint32_t t) {
-        return static_cast<uint32_t>(keys(p, q, t) + BN - 1) / BN;
-    }
+    // keys that tile t's rows see: up to its last row's position
     static __device__ __forceinline__ int32_t keys(const PagedParams& p, const PagedReq& q, uint32_t t) {
         if (!ROWS) return q.len;
         const uint32_t rows = static_cast<uint32_t>(q.n) * p.group;
         const uint32_t last = (min(rows, (t + 1) * ROWS) - 1) / p.group;
         return max(q.len - q.n + static_cast<int32_t>(last) + 1, 0);
     }
-    __device__ __forceinline__ long long border(uint32_t c) const {
-        return total * static_cast<long long>(c) / static_cast<long long>(n_active);
-    }
+    __device__ __forceinline__ long long border(uint32_t c) const { return per * c + min(static_cast<long long>(c), rem); }
     // The key block at which a border at x cuts a unit at [us, us + w) of nb blocks.
     static __device__ __forceinline__ uint32_t cut(long long x, long long us, long long w, uint32_t nb) {
-        if (x >= us + w) return nb;
         const long long y = x - us - kUnitCost;
-        if (y <= 0) return 0;
-        const uint32_t t = static_cast<uint32_t>(y * nb / (w - kUnitCost));
-        return t < kSnap ? 0u : nb - t < kSnap ? nb : t;
+        if (x >= us + w || y >= static_cast<long long>(nb) * BN) return nb;
+        return y <= 0 ? 0u : static_cast<uint32_t>(y) / BN;
+    }
+    // The first CTA whose share ends at x or behind it.
+    __device__ __forceinline__ uint32_t ends_at(long long x) const {
+        uint32_t c = 0;
+        for (uint32_t k = 0; k < n_active; k += 32)
+            c += __popc(__ballot_sync(0xffffffffu, k + lane < n_active && border(k + lane + 1) < x));
+        return c;
     }
 
-    // Every thread of the block: this CTA's share and the request it starts in.  scratch: 40 long longs of
-    // shared memory.  Ends with a block barrier; false: no share.
-    __device__ bool locate(long long* scratch) {
-        const uint32_t tid = threadIdx.x, nt = blockDim.x, nw = nt / 32, warp = tid / 32;
-        lane = static_cast<int>(tid & 31);
+    // This CTA's share and the unit it starts in; false: no share.
+    __device__ bool begin() {
+        lane = static_cast<int>(threadIdx.x & 31);
         cta = blockIdx.x;
-        long long first = 0, sum = 0;   // weight of request tid, and of all of this thread's
-        for (uint32_t i = tid; i < p.n_seqs; i += nt) {
-            const long long w = weight(p, paged_req(p, i));
-            if (i == tid) first = w;
+        long long first = 0, sum = 0;                  // weight of request lane, and of all of this lane's
+        uint32_t units = 0;                            // tiles of a head group
+#pragma unroll 4
+        for (uint32_t i = lane; i < p.n_seqs; i += 32) {
+            const PagedReq q = paged_req(p, i);
+            const long long w = weight(p, q);
+            if (i == static_cast<uint32_t>(lane)) first = w;
             sum += w;
+            units += tiles(p, q);
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) scratch[warp] = sum;
-        __syncthreads();
-        W = 0;
-        for (uint32_t w = 0; w < nw; ++w) W += scratch[w];
+        for (int o = 16; o > 0; o >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            units += __shfl_xor_sync(0xffffffffu, units, o);
+        }
+        W = sum;
+        if (W == 0) return false;
         total = W * p.n_groups;
-        n_active = static_cast<uint32_t>(min(static_cast<long long>(gridDim.x), max(total / kMinShare, 1ll)));
-        if (W == 0 || cta >= n_active) return false;   // the whole block
+        // as many shares as hold kMinShare keys, or a share per unit where that would cut units less than fourfold
+        const long long all = static_cast<long long>(units) * p.n_groups, fine = total / kMinShare;
+        n_active = static_cast<uint32_t>(min(static_cast<long long>(gridDim.x), fine < 4 * all ? all : fine));
+        if (cta >= n_active) return false;
+        per = div_pos(total, n_active);
+        rem = total - per * n_active;
         x0 = border(cta);
         x1 = border(cta + 1);
-        g = static_cast<uint32_t>(x0 / W);
+        g = static_cast<uint32_t>(div_pos(x0, W));
         const long long y = x0 - g * W;
         // the request whose weights hold y
         long long carry = 0;
-        for (uint32_t chunk = 0; chunk < p.n_seqs; chunk += nt) {
-            const uint32_t i = chunk + tid;
-            const long long w = chunk == 0 ? first : i < p.n_seqs ? weight(p, paged_req(p, i)) : 0;
+        bool found = false;
+        auto look = [&](uint32_t chunk, long long w) {
             long long s = w;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const long long u = __shfl_up_sync(0xffffffffu, s, o);
                 if (lane >= o) s += u;
             }
-            __syncthreads();                           // the last round's sums have been read
-            if (lane == 31) scratch[warp] = s;
-            __syncthreads();
-            long long at = carry, all = carry;
-            for (uint32_t k = 0; k < nw; ++k) {
-                if (k < warp) at += scratch[k];
-                all += scratch[k];
+            const uint32_t m = __ballot_sync(0xffffffffu, carry + s > y);
+            if (m) {
+                const int k = __ffs(m) - 1;
+                r = chunk + k;
+                base = carry + __shfl_sync(0xffffffffu, s - w, k);
+                found = true;
+            } else {
+                carry += __shfl_sync(0xffffffffu, s, 31);
             }
-            if (at + s - w <= y && y < at + s) {
-                scratch[32] = i;
-                scratch[33] = at + s - w;
-            }
-            carry = all;
-            if (y < carry) break;                      // uniform: found in this chunk
-        }
-        __syncthreads();
-        r = static_cast<uint32_t>(scratch[32]);
-        base = scratch[33];
+        };
+        for (uint32_t chunk = 0; !found && chunk < p.n_seqs; chunk += 32)
+            look(chunk, chunk == 0 ? first : chunk + lane < p.n_seqs ? weight(p, paged_req(p, chunk + lane)) : 0);
         // the tile of r that holds y: before() grows with t
-        const PagedReq q = paged_req(p, r);
-        uint32_t lo = 0, hi = tiles(p, q);
-        while (hi - lo > 1) {
-            const uint32_t mid = (lo + hi) / 2;
-            if (base + before(p, q, mid) <= y) lo = mid; else hi = mid;
+        j = 0;
+        if (ROWS) {
+            const PagedReq q = paged_req(p, r);
+            uint32_t hi = tiles(p, q);
+            while (hi - j > 1) {
+                const uint32_t mid = (j + hi) / 2;
+                if (base + before(p, q, mid) <= y) j = mid; else hi = mid;
+            }
         }
-        j = lo;
         return true;
     }
 
-    // One warp, all lanes: the next unit of the share into u; false when the share has ended.
+    // The next unit of the share into u; false when the share has ended.
     __device__ bool next(PagedUnit& u) {
         for (;;) {
             if (g >= p.n_groups) return false;
             const PagedReq q = paged_req(p, r);
             const uint32_t nt = tiles(p, q);
             if (j >= nt) {                             // on to the next request that has work
-                base += weight(p, q);
+                base += before(p, q, nt);
                 ++r;
                 j = 0;
                 for (;;) {
@@ -257,10 +322,9 @@ template <int BN, int ROWS> struct PagedSched {
                 }
                 continue;
             }
-            const long long us = g * W + base + before(p, q, j);
-            const long long w = base + before(p, q, j + 1) + g * W - us;
+            const long long at = before(p, q, j), us = g * W + base + at, w = before(p, q, j + 1) - at;
             if (us >= x1) return false;
-            const uint32_t nb = blocks(p, q, j);
+            const uint32_t nb = static_cast<uint32_t>(keys(p, q, j) + BN - 1) / BN;
             u.g = g;
             u.r = r;
             u.j = j++;
@@ -275,20 +339,14 @@ template <int BN, int ROWS> struct PagedSched {
             u.done = 0;
             if (nb == 0) {                             // no key to see: whoever holds its start writes zeros
                 if (us < x0) continue;
+                u.kb0 = u.kb1 = 0;
                 return true;
             }
             if (u.kb0 >= u.kb1) continue;
             if (u.kb0 > 0 || u.kb1 < nb) {
-                // The first piece is the first CTA whose end border cuts past block 0, the last one the first
-                // whose end border cuts at nb; between them every CTA has a piece (kMinShare).
-                const uint32_t ca = static_cast<uint32_t>(max(us * n_active / total - 2, 0ll)) + lane;
-                const bool past = ca < n_active && cut(border(ca + 1), us, w, nb) > 0;
-                const long long tail = max(us + w - (BN + 128) * static_cast<long long>(kSnap), 0ll);
-                const uint32_t cb = static_cast<uint32_t>(max(tail * n_active / total - 3, 0ll)) + lane;
-                const bool whole = cb < n_active && cut(border(cb + 1), us, w, nb) == nb;
-                const uint32_t ma = __ballot_sync(0xffffffffu, past), mb = __ballot_sync(0xffffffffu, whole);
-                u.c_first = __shfl_sync(0xffffffffu, ca, __ffs(ma) - 1);
-                u.n_pieces = __shfl_sync(0xffffffffu, cb, __ffs(mb) - 1) - u.c_first + 1;
+                // the first piece ends where the unit is first cut behind block 0, the last one where nothing is left
+                u.c_first = ends_at(us + min(w, kUnitCost + BN));
+                u.n_pieces = ends_at(us + min(w, kUnitCost + static_cast<long long>(nb) * BN)) - u.c_first + 1;
                 u.slot = 2 * cta + (u.kb0 > 0 ? 0u : 1u);
             }
             return true;

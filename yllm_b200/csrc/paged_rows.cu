@@ -10,7 +10,8 @@
 // ring of stages (K and V of 16 tokens per consumer warp) with tensor copies, one per page and lane: the
 // lanes look the pages up in the block table one stage ahead, so the lookup's latency is off the stream.
 // A copy brings all the unit's dims of min(page, stage) rows (4-D maps); with a copy per 64 dims, 2 KB
-// at 16-row pages, the copies' rate was the bound (64 ragged Llama-3-8B sequences: 232 us against 207).  With a unit's first stage goes its descriptor.  Consumer warps own one kv
+// at 16-row pages, the copies' rate was the bound (64 ragged Llama-3-8B sequences: 232 us against 203).
+// Units are published ahead of their data, so the consumers fetch q while the first stage is in flight.  Consumer warps own one kv
 // head and 16 tokens of each stage; the warps' (m, l, o) meet in the unit's last stage.
 //
 // Bound: HBM, K and V once.
@@ -36,20 +37,23 @@ template <int HD> struct RowsCfg {
     static constexpr int PT_BYTES = 2 * 8 * 48;                  // per warp: P^T hi and lo, 8 rows x 16 tokens
     static constexpr int OFF_PT = NST * STAGE;
     static constexpr int OFF_ML = OFF_PT + NCW * PT_BYTES;       // [NCW][8][2] floats
-    static constexpr int OFF_UNIT = OFF_ML + NCW * 8 * 2 * 4;    // [NST] units, 64 B apart
-    static constexpr int OFF_BAR = OFF_UNIT + NST * 64;
-    static constexpr int OFF_SCRATCH = OFF_BAR + (2 * NST + 2) * 8;   // the schedule's sums; flags before it
-    static constexpr int SMEM = OFF_SCRATCH + 40 * 8 + 1024;     // + alignment slack
+    static constexpr int NU = 4;                                 // unit descriptors in flight
+    static constexpr int OFF_UNIT = OFF_ML + NCW * 8 * 2 * 4;    // [NU] units, 64 B apart
+    static constexpr int OFF_BAR = OFF_UNIT + NU * 64;
+    static constexpr int SMEM = OFF_BAR + (2 * NST + 2 * NU + 2) * 8 + 1024;   // + flags, + alignment slack
     static_assert(sizeof(PagedUnit) <= 64 && SMEM <= 232448, "shared memory");
     static_assert(NCW * 8 * HD * 4 <= STAGE, "the warps' o fit the unit's last stage");
 };
+
+// The two elements of a query row at element offset i, ACT a YATTN_ACT_*.
+template <int ACT> __device__ __forceinline__ float2 q_pair(const void* q, size_t i) { return ld_act2(q, i, ACT); }
 
 template <int HD, int HC>
 __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
     k_paged_rows(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                  const __grid_constant__ PagedParams p) {
     using C = RowsCfg<HD>;
-    constexpr int NCW = C::NCW, NST = C::NST;
+    constexpr int NCW = C::NCW, NST = C::NST, NU = C::NU;
     constexpr int KS = HD / 16;                    // k-steps (QK) and m-tiles (PV)
     constexpr uint32_t TOK = 16u * NCW / HC;       // tokens per stage = keys per block
     constexpr uint32_t TILEB = TOK * HC * HD * 2;
@@ -61,10 +65,12 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
     uint64_t* empty = full + NST;
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + NST);
-    int* last_flag = reinterpret_cast<int*>(empty + NST + 1);
+    uint64_t* u_full = empty + NST;
+    uint64_t* u_empty = u_full + NU;
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(u_empty + NU);
+    int* last_flag = reinterpret_cast<int*>(u_empty + NU + 1);
     float* mrg_ml = reinterpret_cast<float*>(smem + C::OFF_ML);
-    auto unit_at = [&](uint32_t s) { return reinterpret_cast<PagedUnit*>(smem + C::OFF_UNIT + s * 64); };
+    auto unit_at = [&](uint32_t i) { return reinterpret_cast<PagedUnit*>(smem + C::OFF_UNIT + (i % NU) * 64); };
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -72,11 +78,13 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], NCW);
         }
+        for (int s = 0; s < NU; ++s) {
+            mbar_init(&u_full[s], 1);
+            mbar_init(&u_empty[s], NCW);
+        }
         *abort_flag = 0;
         fence_mbar_init();
     }
-    Sched sched(p);
-    if (!sched.locate(reinterpret_cast<long long*>(smem + C::OFF_SCRATCH))) return;   // (has block barriers)
     __syncthreads();
 
     if (warp == NCW) {
@@ -91,14 +99,29 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
         // this lane's copy: K (even) or V (odd) of page lane / 2 of the stage (8 pages at most)
         const uint32_t i_pg = lane >> 1, i_v = lane & 1;
         const bool mine = i_pg < per_block;
-        uint32_t gi = 0;
+        uint32_t gi = 0, ui = 0;
         bool ok = true;
+        Sched sched(p);
+        auto publish = [&](const PagedUnit& u) -> bool {
+            if (ui >= static_cast<uint32_t>(NU) &&
+                !warp_wait_bounded(&u_empty[ui % NU], ((ui / NU) & 1u) ^ 1u, p.status, ST_PAGED_TIMEOUT, abort_flag))
+                return false;
+            if (lane == 0) {
+                *unit_at(ui) = u;
+                mbar_arrive(&u_full[ui % NU]);
+            }
+            ++ui;
+            return true;
+        };
         PagedUnit u;
         auto claim = [&](uint32_t s) -> bool {
             return gi < static_cast<uint32_t>(NST) ||
                    warp_wait_bounded(&empty[s], ((gi / NST) & 1u) ^ 1u, p.status, ST_PAGED_TIMEOUT, abort_flag);
         };
-        while (ok && sched.next(u)) {
+        const bool share = sched.begin();
+        while (ok && share && sched.next(u)) {
+            ok = publish(u);
+            if (!ok) break;
             const uint32_t nt = max(1u, u.kb1 - u.kb0);
             const int32_t pan0 = static_cast<int32_t>(u.g * NPAN);
             // row of this lane's copy in block b, or -1 behind the request's last key
@@ -114,7 +137,6 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                     ok = false;
                     break;
                 }
-                if (i == 0 && lane == 0) *unit_at(s) = u;     // published by the arrive on full[s]
                 const uint32_t n_copy = __popc(__ballot_sync(0xffffffffu, row >= 0));
                 if (lane == 0) mbar_arrive_expect_tx(&full[s], n_copy * box * (NPAN * 128));
                 __syncwarp();
@@ -124,16 +146,8 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                 row = i + 1 < nt ? row_of(u.kb0 + i + 1) : -1;
             }
         }
-        if (ok) {                                             // the end of the list
-            const uint32_t s = gi % NST;
-            if (claim(s)) {
-                if (lane == 0) {
-                    unit_at(s)->done = 1;
-                    mbar_arrive(&full[s]);
-                }
-                ++gi;
-            }
-        }
+        u.done = 1;
+        if (ok) publish(u);                                   // the end of the list
         // no copy may still be in flight when the CTA exits (consumers stop early on an abort)
         volatile int dummy = 0;
         for (uint32_t b = gi > static_cast<uint32_t>(NST) ? gi - NST : 0; b < gi; ++b)
@@ -160,12 +174,17 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                ((static_cast<uint32_t>(((mt & 3) << 1) + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
     };
 
+    // query rows of a kv head: row f is token f / group, head f % group.  This lane's row of the Q fragment (g8)
+    // and of S^T's columns (2 t4, 2 t4 + 1)
+    const uint32_t tok_q = g8 / p.group, head_q = g8 % p.group;
+    const int32_t tok_a = 2 * t4 / p.group, tok_b = (2 * t4 + 1) / p.group;
     uint32_t tb = 0;   // stages of this CTA's earlier units
-    for (;;) {
-        const uint32_t s0 = tb % NST;
-        const bool got = warp_wait_bounded(&full[s0], (tb / NST) & 1u, p.status, ST_PAGED_TIMEOUT, abort_flag);
+    for (uint32_t ui = 0;; ++ui) {
+        const bool got = warp_wait_bounded(&u_full[ui % NU], (ui / NU) & 1u, p.status, ST_PAGED_TIMEOUT, abort_flag);
         if (!named_bar_and(1, 32 * NCW, got)) return;
-        const PagedUnit u = *unit_at(s0);
+        const PagedUnit u = *unit_at(ui);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&u_empty[ui % NU]);
         if (u.done) return;
         const uint32_t nt = max(1u, u.kb1 - u.kb0);
         const uint32_t rows = static_cast<uint32_t>(u.n) * p.group;            // query rows per kv head, <= 8
@@ -176,19 +195,20 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
         float up;
         {
             const bool hv = static_cast<uint32_t>(g8) < rows;
-            const uint32_t f = hv ? g8 : 0;
-            const size_t qa = (u.tok0 + static_cast<size_t>(f / p.group)) * p.q_stride +
-                              static_cast<size_t>(head0 + f % p.group) * HD + 2 * t4;
+            const size_t qa = (u.tok0 + static_cast<size_t>(hv ? tok_q : 0)) * p.q_stride +
+                              static_cast<size_t>(head0 + (hv ? head_q : 0)) * HD + 2 * t4;
             float2 xa[KS], xb[KS];
             float mx = 0.f;
+            auto load = [&](auto pair) {
 #pragma unroll
-            for (int kk = 0; kk < KS; ++kk) {
-                xa[kk] = xb[kk] = make_float2(0.f, 0.f);
-                if (hv) {
-                    xa[kk] = ld_act2(p.q, qa + kk * 16, p.act);
-                    xb[kk] = ld_act2(p.q, qa + kk * 16 + 8, p.act);
+                for (int kk = 0; kk < KS; ++kk) {
+                    xa[kk] = hv ? pair(qa + kk * 16) : make_float2(0.f, 0.f);
+                    xb[kk] = hv ? pair(qa + kk * 16 + 8) : make_float2(0.f, 0.f);
                 }
-            }
+            };
+            if (p.act == YATTN_ACT_F32) load([&](size_t i) { return q_pair<YATTN_ACT_F32>(p.q, i); });
+            else if (p.act == YATTN_ACT_F16) load([&](size_t i) { return q_pair<YATTN_ACT_F16>(p.q, i); });
+            else load([&](size_t i) { return q_pair<YATTN_ACT_BF16>(p.q, i); });
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk)
                 mx = fmaxf(mx, fmaxf(fmaxf(fabsf(xa[kk].x), fabsf(xa[kk].y)), fmaxf(fabsf(xb[kk].x), fabsf(xb[kk].y))));
@@ -202,12 +222,12 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                 split_h2(xb[kk].x * down, xb[kk].y * down, qhi[kk][1], qlo[kk][1]);
             }
         }
-        // columns of S^T: rows 2 t4 and 2 t4 + 1; how many keys each sees
+        // columns of S^T: how many keys each sees
         const float sc_a = p.scale_log2 * __shfl_sync(0xffffffffu, up, 8 * t4);
         const float sc_b = p.scale_log2 * __shfl_sync(0xffffffffu, up, 8 * t4 + 4);
         const int32_t seen0 = u.len - u.n + 1;
-        const int32_t see_a = static_cast<uint32_t>(2 * t4) < rows ? seen0 + static_cast<int32_t>(2 * t4 / p.group) : 0;
-        const int32_t see_b = static_cast<uint32_t>(2 * t4 + 1) < rows ? seen0 + static_cast<int32_t>((2 * t4 + 1) / p.group) : 0;
+        const int32_t see_a = static_cast<uint32_t>(2 * t4) < rows ? seen0 + tok_a : 0;
+        const int32_t see_b = static_cast<uint32_t>(2 * t4 + 1) < rows ? seen0 + tok_b : 0;
 
         float oc[KS][4];
 #pragma unroll
@@ -216,7 +236,7 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
 
         for (uint32_t i = 0; i < nt; ++i) {
             const uint32_t gi = tb + i, s = gi % NST;
-            if (i > 0 && !warp_wait_bounded(&full[s], (gi / NST) & 1u, p.status, ST_PAGED_TIMEOUT, abort_flag)) break;
+            if (!warp_wait_bounded(&full[s], (gi / NST) & 1u, p.status, ST_PAGED_TIMEOUT, abort_flag)) break;
             const int32_t key0 = static_cast<int32_t>((u.kb0 + i) * TOK + 16 * sl);   // this warp's first key
             const int nvalid = u.kb1 > u.kb0 ? max(0, min(16, u.len - key0)) : 0;
             if (nvalid > 0) {
@@ -334,40 +354,51 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
             }
         }
         named_bar_sync(1, 32 * NCW);
-        constexpr int DPL = HD / 32;
+        constexpr int DPL = HD / 32;                          // dims [lane * DPL, +DPL) of a row are this lane's
         const bool whole = u.n_pieces == 1;
-        // one warp per (kv head, query row); lane owns dims lane + 32 i
+        // one warp per (kv head, query row)
         auto finish = [&](uint32_t h, uint32_t f, const float (&acc)[DPL], float l) {
             const float inv = l == 0.f ? 0.f : 1.0f / l;      // no key seen: zeros
-            const size_t tok = u.tok0 + static_cast<size_t>(f / p.group);
-            const size_t col = static_cast<size_t>((u.g * HC + h) * p.group + f % p.group) * HD + lane;
+            const uint32_t tk = f / p.group;
+            const size_t tok = u.tok0 + static_cast<size_t>(tk);
+            const size_t col = static_cast<size_t>((u.g * HC + h) * p.group + f - tk * p.group) * HD + lane * DPL;
+            float x[DPL];
 #pragma unroll
-            for (int i = 0; i < DPL; ++i) {
-                float x = acc[i] * inv;
-                if (p.gate) x *= sigmoid_of(ld_act(p.gate, tok * p.gate_stride + col + 32 * i, p.act));
-                st_act(p.out, tok * p.out_stride + col + 32 * i, p.act, x);
+            for (int i = 0; i < DPL; ++i) x[i] = acc[i] * inv;
+            if (p.gate) {
+#pragma unroll
+                for (int i = 0; i < DPL; i += 2) {
+                    const float2 g = ld_act2(p.gate, tok * p.gate_stride + col + i, p.act);
+                    x[i] *= sigmoid_of(g.x);
+                    x[i + 1] *= sigmoid_of(g.y);
+                }
             }
+            st_act_vec<DPL>(p.out, tok * p.out_stride + col, p.act, x);
         };
         for (uint32_t row = warp; row < HC * rows; row += NCW) {
-            const uint32_t h = row / rows, f = row % rows;
-            float M = -INFINITY, l = 0.f, acc[DPL];
-            for (uint32_t j = 0; j < NSL; ++j) M = fmaxf(M, mrg_ml[((h + j * HC) * 8 + f) * 2]);
+            const uint32_t h = row >= rows ? 1 : 0, f = row - h * rows;          // HC <= 2
+            float M = -INFINITY, l = 0.f, acc[DPL], mw[NSL], o[DPL];
+#pragma unroll
+            for (uint32_t j = 0; j < NSL; ++j) {
+                mw[j] = mrg_ml[((h + j * HC) * 8 + f) * 2];
+                M = fmaxf(M, mw[j]);
+            }
 #pragma unroll
             for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
-            for (uint32_t j = 0; j < NSL; ++j) {
-                const uint32_t w = h + j * HC;
-                const float mw = mrg_ml[(w * 8 + f) * 2];
-                const float sc = mw == -INFINITY ? 0.f : ex2_approx(mw - M);
-                l += sc * mrg_ml[(w * 8 + f) * 2 + 1];
 #pragma unroll
-                for (int i = 0; i < DPL; ++i) acc[i] += sc * mrg_o[(w * 8 + f) * HD + lane + 32 * i];
+            for (uint32_t j = 0; j < NSL; ++j) {
+                const uint32_t at = (h + j * HC) * 8 + f;
+                const float sc = mw[j] == -INFINITY ? 0.f : ex2_approx(mw[j] - M);
+                l += sc * mrg_ml[at * 2 + 1];
+                ld_vec<DPL>(mrg_o + at * HD + lane * DPL, o);
+#pragma unroll
+                for (int i = 0; i < DPL; ++i) acc[i] += sc * o[i];
             }
             if (whole) {
                 finish(h, f, acc, l);
             } else {
                 const size_t at = static_cast<size_t>(u.slot) * (HC * 8) + h * 8 + f;
-#pragma unroll
-                for (int i = 0; i < DPL; ++i) p.part_o[at * HD + lane + 32 * i] = acc[i];
+                st_vec<DPL>(p.part_o + at * HD + lane * DPL, acc);
                 if (lane == 0) *reinterpret_cast<float2*>(&p.part_ml[at * 2]) = make_float2(M, l);
             }
         }
@@ -385,10 +416,12 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
         if (!*last_flag) continue;
         __threadfence();
         for (uint32_t row = warp; row < HC * rows; row += NCW) {
-            const uint32_t h = row / rows, f = row % rows;
+            const uint32_t h = row >= rows ? 1 : 0, f = row - h * rows;
+            // row (h, f) of piece i: slot 2 c_first + 1, then every second one from 2 (c_first + 1)
             auto at = [&](uint32_t i) { return static_cast<size_t>(piece_slot(u.c_first, i)) * (HC * 8) + h * 8 + f; };
             float2 ml[kPagedMaxPieces / 32];          // lane: pieces lane, lane + 32, ..
-            float M = -INFINITY, l = 0.f, acc[DPL];
+            float M = -INFINITY, l = 0.f, acc[DPL], o0[DPL];
+            ldcg_vec_n<DPL>(p.part_o + at(0) * HD + lane * DPL, o0);
 #pragma unroll
             for (int c = 0; c < kPagedMaxPieces / 32; ++c) {
                 const uint32_t i = c * 32 + lane;
@@ -398,32 +431,39 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-#pragma unroll
-            for (int i = 0; i < DPL; ++i) acc[i] = 0.f;
+            float w[kPagedMaxPieces / 32];
 #pragma unroll
             for (int c = 0; c < kPagedMaxPieces / 32; ++c) {
-                const float w = ml[c].x == -INFINITY ? 0.f : ex2_approx(ml[c].x - M);
-                l += w * ml[c].y;
-                const uint32_t n = c * 32u < u.n_pieces ? min(32u, u.n_pieces - c * 32u) : 0u;
-                for (uint32_t k = 0; k < n; k += 4) {  // four pieces' loads in flight
-                    float o[4][DPL];
-#pragma unroll
-                    for (int y = 0; y < 4; ++y)
-#pragma unroll
-                        for (int i = 0; i < DPL; ++i)
-                            o[y][i] = k + y < n ? __ldcg(&p.part_o[at(c * 32 + k + y) * HD + lane + 32 * i]) : 0.f;
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        const float wy = __shfl_sync(0xffffffffu, w, (k + y) & 31);
-                        if (k + y < n) {
-#pragma unroll
-                            for (int i = 0; i < DPL; ++i) acc[i] += wy * o[y][i];
-                        }
-                    }
-                }
+                w[c] = ml[c].x == -INFINITY ? 0.f : ex2_approx(ml[c].x - M);
+                l += w[c] * ml[c].y;
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            const float w0 = __shfl_sync(0xffffffffu, w[0], 0);
+#pragma unroll
+            for (int i = 0; i < DPL; ++i) acc[i] = w0 * o0[i];
+            constexpr uint32_t FLY = 32 / DPL;         // pieces' loads in flight
+            constexpr uint32_t STEP = 2 * HC * 8 * HD; // floats between consecutive pieces
+            const float* src = p.part_o + at(1) * HD + lane * DPL;
+#pragma unroll
+            for (int c = 0; c < kPagedMaxPieces / 32; ++c) {
+                for (uint32_t k = c * 32u; k < min(u.n_pieces, c * 32u + 32u); k += FLY) {   // pieces [k, k + FLY)
+                    float o[FLY][DPL];
+#pragma unroll
+                    for (uint32_t y = 0; y < FLY; ++y) {
+#pragma unroll
+                        for (int i = 0; i < DPL; ++i) o[y][i] = 0.f;
+                        if (k + y >= 1 && k + y < u.n_pieces)
+                            ldcg_vec_n<DPL>(src + static_cast<size_t>(k) * STEP + static_cast<int>(y - 1) * static_cast<int>(STEP), o[y]);
+                    }
+#pragma unroll
+                    for (uint32_t y = 0; y < FLY; ++y) {
+                        const float wy = __shfl_sync(0xffffffffu, w[c], (k + y) & 31);
+#pragma unroll
+                        for (int i = 0; i < DPL; ++i) acc[i] += wy * o[y][i];
+                    }
+                }
+            }
             finish(h, f, acc, l);
         }
     }

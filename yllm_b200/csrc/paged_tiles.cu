@@ -43,8 +43,7 @@ template <int HD> struct TCfg {
     static constexpr int OFF_V = OFF_K + KST * KV_BYTES;
     static constexpr int OFF_X = OFF_V + VST * KV_BYTES;    // [2 blocks][2 halves][BM] floats: row maxima / sums
     static constexpr int OFF_U = OFF_X + 2 * 2 * BM * 4;    // [NU] units, 64 B apart
-    static constexpr int OFF_SCRATCH = OFF_U + NU * 64;     // the schedule's sums
-    static constexpr int OFF_BAR = OFF_SCRATCH + 40 * 8;
+    static constexpr int OFF_BAR = OFF_U + NU * 64;
     static constexpr int SMEM = OFF_BAR + 320 + 1024;       // + barriers, + alignment slack
     static constexpr uint32_t TMEM_COLS = 512;
     static constexpr uint32_t COL_S = 0;                    // S buffer b at [b*BN, (b+1)*BN)
@@ -118,8 +117,6 @@ __global__ void __launch_bounds__(kTThreads, 1)
         bars->abort_flag = 0;
         fence_mbar_init();
     }
-    Sched sched(p);
-    if (!sched.locate(reinterpret_cast<long long*>(smem + C::OFF_SCRATCH))) return;   // the whole block
     if (warp == 0) tmem_alloc(&bars->tmem_base, C::TMEM_COLS);
     tc_fence_before();
     __syncthreads();
@@ -142,10 +139,11 @@ __global__ void __launch_bounds__(kTThreads, 1)
     if (warp == 11) {
         // ================= schedule =================
         uint32_t ui = 0;
-        bool ok = true, more = true;
-        while (ok && more) {
+        Sched sched(p);
+        bool ok = true, more = sched.begin();
+        for (;;) {
             PagedUnit u;
-            more = sched.next(u);
+            more = more && sched.next(u);
             if (ui >= NU)
                 ok = warp_wait_bounded(&bars->u_empty[ui % NU], ((ui / NU) & 1u) ^ 1u, status, ST_PAGED_TIMEOUT, abort_flag);
             if (ok && lane == 0) {
@@ -153,6 +151,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 *unit_at(ui) = u;
                 mbar_arrive(&bars->u_full[ui % NU]);
             }
+            if (!ok || !more) break;
             ++ui;
         }
     } else if (warp == 8 || warp == 10) {
