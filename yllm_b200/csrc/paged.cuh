@@ -29,12 +29,13 @@ struct PagedParams {
     uint32_t table_stride, max_pages, n_pages, page_shift;
     uint32_t n_tokens, n_seqs, max_new;
     uint32_t n_heads, group;          // query heads, query heads per kv head
+    uint32_t group_m, group_s;        // x / group = x * group_m >> group_s for x < 2^31
     uint32_t hc, n_groups;            // kv heads per unit, units' head groups (n_kv / hc)
     int act;                          // YATTN_ACT_*
     float scale_log2;                 // log2(e) / sqrt(head_dim)
     uint32_t* counters;               // [gridDim.x]: pieces of a cut unit that are done, by its first CTA
     float* part_ml;                   // [2 * gridDim.x][rows][2]
-    float* part_o;                    // [2 * gridDim.x][rows][HD]
+    float* part_o;                    // [3 * gridDim.x][rows][HD]: two partials a CTA, then a folded sum each
     int* status;
 };
 
@@ -127,6 +128,10 @@ __device__ __forceinline__ void row_scale(float mx, float& down, float& up) {
     up = __uint_as_float(e << 23);
 }
 
+__device__ __forceinline__ uint32_t div_group(const PagedParams& p, uint32_t x) {
+    return static_cast<uint32_t>(static_cast<uint64_t>(x) * p.group_m >> p.group_s);
+}
+
 // ------------------------------------------------------------------ requests
 
 struct PagedReq {
@@ -164,6 +169,7 @@ struct PagedUnit {
     uint32_t n_pieces;          // 1: the unit is whole
     uint32_t c_first;           // CTA of the unit's first piece
     uint32_t slot;              // this piece's partial slot
+    int32_t keys;               // keys that the tile's last row sees
     uint32_t done;              // 1: no unit, the list has ended
 };
 
@@ -174,14 +180,17 @@ __device__ __forceinline__ long long div_pos(long long a, long long b) {
 }
 
 // ROWS: query rows per tile (a row is one token x one head of the group); 0: a request's rows are one tile.
-// One warp runs it, all lanes.
+// One warp runs it, all lanes.  Weights are in units of 1 / group key where ROWS, so that no sum needs a division.
 template <int BN, int ROWS> struct PagedSched {
-    // Keys charged for a unit besides its own, and the least keys of a share where units are cut.  A cut costs a
-    // partial's round trip through memory, about 2.5 us, and a block of the decode form 0.9 us when nothing else
-    // runs: shares of 128 beat 512 there from 512 keys on (one Llama-3-8B sequence, 1024 keys: 12.0 us against
-    // 17.6), and cutting a unit less than about fourfold loses (256 keys: 12.0 us cut, 11.1 whole).
-    static constexpr long long kUnitCost = ROWS ? 384 : 192;
-    static constexpr long long kMinShare = ROWS ? 256 : 128;
+    // Keys charged for a unit besides its own, the least keys of a share where units are cut, the least blocks of a
+    // cut unit's first and last piece.  A cut costs a partial's round trip through memory.  Decode form: about
+    // 2.5 us, and a block 0.9 us when nothing else runs: shares of 128 beat 512 from 512 keys on (one Llama-3-8B
+    // sequence, 1024 keys: 12.0 us against 17.6), and cutting a unit less than about fourfold loses (256 keys:
+    // 12.0 us cut, 11.1 whole).
+    static constexpr long long kUnitCost = ROWS ? 512 : 192;
+    static constexpr long long kMinShare = ROWS ? 512 : 128;
+    static constexpr uint32_t kSnap = ROWS ? 256 / BN : 1;
+    static constexpr long long kCutFrom = ROWS ? 2 : 4;   // cut where a unit would get that many shares on average
     static_assert(kUnitCost >= BN && kMinShare >= BN, "a share inside a unit holds a block, so a cut unit's pieces are contiguous CTAs");
 
     const PagedParams& p;
@@ -193,6 +202,8 @@ template <int BN, int ROWS> struct PagedSched {
 
     __device__ __forceinline__ explicit PagedSched(const PagedParams& pp) : p(pp) {}
 
+    static __device__ __forceinline__ long long unit_cost(const PagedParams& p) { return ROWS ? kUnitCost * p.group : kUnitCost; }
+    static __device__ __forceinline__ long long block_cost(const PagedParams& p) { return ROWS ? BN * static_cast<long long>(p.group) : BN; }
     static __device__ __forceinline__ uint32_t tiles(const PagedParams& p, const PagedReq& q) {
         if (!ROWS) return q.n > 0 ? 1u : 0u;
         return (static_cast<uint32_t>(q.n) * p.group + ROWS - 1) / (ROWS ? ROWS : 1);
@@ -201,7 +212,7 @@ template <int BN, int ROWS> struct PagedSched {
     static __device__ __forceinline__ long long before(const PagedParams& p, const PagedReq& q, uint32_t t) {
         if (!ROWS) return t ? kUnitCost + q.len : 0;
         const long long T = t;
-        return T * (kUnitCost + max(q.len - q.n, 0)) + div_pos(T * (T + 1) * (ROWS / 2), p.group);
+        return T * ((kUnitCost + max(q.len - q.n, 0)) * p.group) + T * (T + 1) * (ROWS / 2);
     }
     static __device__ __forceinline__ long long weight(const PagedParams& p, const PagedReq& q) {
         return before(p, q, tiles(p, q));
@@ -210,15 +221,16 @@ template <int BN, int ROWS> struct PagedSched {
     static __device__ __forceinline__ int32_t keys(const PagedParams& p, const PagedReq& q, uint32_t t) {
         if (!ROWS) return q.len;
         const uint32_t rows = static_cast<uint32_t>(q.n) * p.group;
-        const uint32_t last = (min(rows, (t + 1) * ROWS) - 1) / p.group;
+        const uint32_t last = div_group(p, min(rows, (t + 1) * ROWS) - 1);
         return max(q.len - q.n + static_cast<int32_t>(last) + 1, 0);
     }
     __device__ __forceinline__ long long border(uint32_t c) const { return per * c + min(static_cast<long long>(c), rem); }
     // The key block at which a border at x cuts a unit at [us, us + w) of nb blocks.
-    static __device__ __forceinline__ uint32_t cut(long long x, long long us, long long w, uint32_t nb) {
-        const long long y = x - us - kUnitCost;
-        if (x >= us + w || y >= static_cast<long long>(nb) * BN) return nb;
-        return y <= 0 ? 0u : static_cast<uint32_t>(y) / BN;
+    __device__ __forceinline__ uint32_t cut(long long x, long long us, long long w, uint32_t nb) const {
+        const long long y = x - us - unit_cost(p);
+        if (x >= us + w || y >= static_cast<long long>(nb) * block_cost(p)) return nb;
+        const uint32_t t = y <= 0 ? 0u : static_cast<uint32_t>(ROWS ? div_pos(y, block_cost(p)) : y / BN);
+        return t < kSnap ? 0u : nb - t < kSnap ? nb : t;
     }
     // The first CTA whose share ends at x or behind it.
     __device__ __forceinline__ uint32_t ends_at(long long x) const {
@@ -250,9 +262,9 @@ template <int BN, int ROWS> struct PagedSched {
         W = sum;
         if (W == 0) return false;
         total = W * p.n_groups;
-        // as many shares as hold kMinShare keys, or a share per unit where that would cut units less than fourfold
-        const long long all = static_cast<long long>(units) * p.n_groups, fine = total / kMinShare;
-        n_active = static_cast<uint32_t>(min(static_cast<long long>(gridDim.x), fine < 4 * all ? all : fine));
+        // as many shares as hold kMinShare keys, or a share per unit where that would cut units into fewer than kCutFrom
+        const long long all = static_cast<long long>(units) * p.n_groups, fine = ROWS ? div_pos(total, kMinShare * p.group) : total / kMinShare;
+        n_active = static_cast<uint32_t>(min(static_cast<long long>(gridDim.x), fine < kCutFrom * all ? all : fine));
         if (cta >= n_active) return false;
         per = div_pos(total, n_active);
         rem = total - per * n_active;
@@ -324,7 +336,8 @@ template <int BN, int ROWS> struct PagedSched {
             }
             const long long at = before(p, q, j), us = g * W + base + at, w = before(p, q, j + 1) - at;
             if (us >= x1) return false;
-            const uint32_t nb = static_cast<uint32_t>(keys(p, q, j) + BN - 1) / BN;
+            u.keys = keys(p, q, j);
+            const uint32_t nb = static_cast<uint32_t>(u.keys + BN - 1) / BN;
             u.g = g;
             u.r = r;
             u.j = j++;
@@ -345,8 +358,9 @@ template <int BN, int ROWS> struct PagedSched {
             if (u.kb0 >= u.kb1) continue;
             if (u.kb0 > 0 || u.kb1 < nb) {
                 // the first piece ends where the unit is first cut behind block 0, the last one where nothing is left
-                u.c_first = ends_at(us + min(w, kUnitCost + BN));
-                u.n_pieces = ends_at(us + min(w, kUnitCost + static_cast<long long>(nb) * BN)) - u.c_first + 1;
+                const long long uc = unit_cost(p), bc = block_cost(p);
+                u.c_first = ends_at(us + min(w, uc + kSnap * bc));
+                u.n_pieces = ends_at(us + min(w, uc + max(kSnap, nb - kSnap + 1) * bc)) - u.c_first + 1;
                 u.slot = 2 * cta + (u.kb0 > 0 ? 0u : 1u);
             }
             return true;

@@ -6,12 +6,12 @@
 namespace yattn {
 namespace {
 
-// Workspace: kPagedCounters counters (zero between calls), then per slot (two per CTA) the partial rows'
-// (m, l) and o.  The tiles kernel's slots are the larger ones.
+// Workspace: kPagedCounters counters (zero between calls), then the partial rows' (m, l), two slots per CTA, and
+// o, two slots per CTA and one for the folded sums.  The tiles kernel's slots are the larger ones.
 size_t ml_offset() { return kPagedCounters * sizeof(uint32_t); }
 size_t workspace_bytes(uint32_t hd) {
-    const size_t slots = 2 * static_cast<size_t>(std::min<uint32_t>(static_cast<uint32_t>(dev_num_sms()), kPagedMaxPieces));
-    return ml_offset() + slots * kPagedTileRows * (2 + static_cast<size_t>(hd)) * sizeof(float);
+    const size_t ctas = std::min<uint32_t>(static_cast<uint32_t>(dev_num_sms()), kPagedMaxPieces);
+    return ml_offset() + ctas * kPagedTileRows * (2 * 2 + 3 * static_cast<size_t>(hd)) * sizeof(float);
 }
 
 int attn_paged(void* out, uint32_t out_stride, const void* q, uint32_t q_stride, const void* gate,
@@ -99,6 +99,11 @@ int attn_paged(void* out, uint32_t out_stride, const void* q, uint32_t q_stride,
     p.max_new = std::min(max_new, n_tokens);
     p.n_heads = n_heads;
     p.group = n_heads / n_kv;
+    // x / d = x * ceil(2^(31 + l) / d) >> (31 + l) for x < 2^31, l = ceil(log2 d)
+    uint32_t l = 0;
+    while ((1u << l) < p.group) ++l;
+    p.group_s = 31 + l;
+    p.group_m = static_cast<uint32_t>(((1ull << p.group_s) + p.group - 1) / p.group);
     p.act = act;
     p.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(hd));
     p.counters = static_cast<uint32_t*>(ws);

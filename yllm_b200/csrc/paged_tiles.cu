@@ -7,12 +7,16 @@
 // fp32 activations (PREC): q = hi + lo and P = hi + lo in fp16, four products for about 22 bits.  16-bit
 // activations: one plane of each (fp16 holds their q exactly; P's half step 2^-11 is below the output's own
 // rounding at bf16 and equal to it at fp16).  Each q row is scaled by a power of two into (-2, 2) first,
-// and P carries a factor 2^7 (it cancels in O / l): see row_scale() and kPUp.
+// and P carries a factor 2^7 (it cancels in O / l): see row_scale() and kPUp.  The tensor core truncates where
+// it adds to an accumulator, always towards zero, so PREC sums at most 1024 keys in one and adds those sums
+// in fp32 (fold() below): over 8700 keys the error was 1.1e-5 of the result without it.
 //
 // One persistent CTA per SM walks its share of the schedule (paged.cuh).  Warps:
 //   0-7  softmax: row r of the tile (TMEM lane r) belongs to warps r/32 and r/32 + 4, which halve each
-//        block's columns.  They fetch Q (hi to shared memory, lo to TMEM), turn S into P in place, rescale
-//        O when m grows by more than 2^8, and write the unit's rows or partials.
+//        block's columns.  They fetch Q, turn S into P in place, rescale O when m grows by more than 2^8,
+//        and write the unit's rows or partials.  Rows are fetched and written through a warp's 2 KB of
+//        shared memory, whole 64-byte runs at a time: with a row per lane every access touched 32 lines,
+//        and a gated unit at head_dim 256 spent 12 us on its way out.
 //   8, 10  K and V blocks by tensor copies into their rings, one copy per page and lane (4-D maps).
 //   9    MMA issue.  S runs up to NSB blocks ahead of the softmax.
 //   11   the schedule: units into a ring of four descriptors, so finding the next unit is off the others' path.
@@ -32,31 +36,34 @@ constexpr int NU = 4;                    // unit descriptors in flight
 // P's factor: m may be stale by 8 binades, and fp16 ends below 2^16
 constexpr float kPUp = 7.f;
 
-template <int HD> struct TCfg {
+template <int HD, bool PREC> struct TCfg {
     static constexpr int BN = HD >= 256 ? 64 : 128;
-    static constexpr int KST = HD >= 256 ? 2 : 3;           // K ring depth
+    static constexpr bool LO_SMEM = PREC && HD <= 128;      // Q_lo in shared memory; head_dim 256: in TMEM
+    static constexpr int KST = HD >= 256 || (HD == 128 && PREC) ? 2 : 3;    // K ring depth
     static constexpr int VST = HD >= 128 ? 2 : 3;           // V ring depth: V(j) is needed two blocks after K(j)
     static constexpr int Q_BYTES = BM * HD * 2;
     static constexpr int KV_BYTES = BN * HD * 2;
     static constexpr int OFF_Q = 0;
-    static constexpr int OFF_K = OFF_Q + Q_BYTES;
+    static constexpr int OFF_QLO = OFF_Q + Q_BYTES;
+    static constexpr int OFF_K = OFF_QLO + (LO_SMEM ? Q_BYTES : 0);
     static constexpr int OFF_V = OFF_K + KST * KV_BYTES;
-    static constexpr int OFF_X = OFF_V + VST * KV_BYTES;    // [2 blocks][2 halves][BM] floats: row maxima / sums
-    static constexpr int OFF_U = OFF_X + 2 * 2 * BM * 4;    // [NU] units, 64 B apart
+    static constexpr int OFF_STG = OFF_V + VST * KV_BYTES;  // per softmax warp: 32 rows x 64 B
+    static constexpr int OFF_X = OFF_STG + 8 * 2048;        // [2 blocks][2 halves][BM] floats: row maxima / sums
+    static constexpr int OFF_UP = OFF_X + 2 * 2 * BM * 4;   // [BM] floats: the rows' powers of two
+    static constexpr int OFF_U = OFF_UP + BM * 4;           // [NU] units, 64 B apart
     static constexpr int OFF_BAR = OFF_U + NU * 64;
     static constexpr int SMEM = OFF_BAR + 320 + 1024;       // + barriers, + alignment slack
     static constexpr uint32_t TMEM_COLS = 512;
-    static constexpr uint32_t COL_S = 0;                    // S buffer b at [b*BN, (b+1)*BN)
-    static constexpr uint32_t COL_O = 3 * BN;
-    static_assert(3 * BN + HD <= static_cast<int>(TMEM_COLS), "TMEM columns");
-    // Q_lo (PREC), HD/2 columns: after O at head_dim 64, in the third S buffer (then after O) above
-    static constexpr int NSB_LO = HD == 64 ? 3 : 2;
-    __host__ __device__ static constexpr uint32_t qlo_col(int kk) {
-        return HD == 64 ? COL_O + HD + 8u * kk
-             : HD == 128 ? 2u * BN + 8u * kk
-             : (kk < 8 ? 2u * BN + 8u * kk : COL_O + HD + 8u * (kk - 8));
-    }
-    static_assert(qlo_col(HD / 16 - 1) + 8 <= TMEM_COLS, "Q_lo columns");
+    static constexpr int NSB = PREC ? 2 : 3;                // S buffers: b at columns [b*BN, (b+1)*BN)
+    static constexpr uint32_t COL_S = 0;
+    static constexpr uint32_t COL_QLO = NSB * BN;           // head_dim 256, PREC: HD/2 columns
+    static constexpr uint32_t COL_O = PREC ? 256 : NSB * BN;
+    // PREC: the fp32 sum of the folded O.  Beside O, or at head_dim 256, where TMEM is full, in global memory
+    static constexpr bool FOLD_TMEM = HD <= 128;
+    static constexpr uint32_t COL_F = COL_O + HD;
+    static constexpr uint32_t FOLD = 1024 / BN;             // blocks per fold
+    static_assert(COL_O + HD * (PREC && FOLD_TMEM ? 2 : 1) <= TMEM_COLS && NSB * BN <= static_cast<int>(COL_O), "TMEM columns");
+    static_assert(!PREC || LO_SMEM || COL_QLO + HD / 2 <= COL_O, "Q_lo columns");
     static_assert(SMEM <= 232448 && sizeof(PagedUnit) <= 64, "shared memory");
 };
 
@@ -71,13 +78,46 @@ template <int KST, int VST> struct TBars {
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
+// A warp's 32 rows of 64 bytes through 2 KB of shared memory, 16-byte chunk c of row r at c ^ (r / 2 & 3): from
+// four lanes a row (lane: rows lane / 4 + 8 i) to a row per lane, and back.
+__device__ __forceinline__ void stage_in(uint8_t* stg, int lane, const uint4 (&raw)[4], uint32_t (&w)[16]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int rr = i * 8 + (lane >> 2);
+        *reinterpret_cast<uint4*>(stg + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4)) = raw[i];
+    }
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint4 v = *reinterpret_cast<const uint4*>(stg + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4));
+        w[4 * k] = v.x;
+        w[4 * k + 1] = v.y;
+        w[4 * k + 2] = v.z;
+        w[4 * k + 3] = v.w;
+    }
+    __syncwarp();
+}
+__device__ __forceinline__ void stage_out(uint8_t* stg, int lane, const uint32_t (&w)[16], uint4 (&raw)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        *reinterpret_cast<uint4*>(stg + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) =
+            make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int rr = i * 8 + (lane >> 2);
+        raw[i] = *reinterpret_cast<const uint4*>(stg + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
+    }
+    __syncwarp();
+}
+
 template <int HD, bool PREC>
 __global__ void __launch_bounds__(kTThreads, 1)
     k_paged_tiles(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const __grid_constant__ PagedParams p) {
-    using C = TCfg<HD>;
+    using C = TCfg<HD, PREC>;
     constexpr int BN = C::BN, HB = BN / 2, KST = C::KST, VST = C::VST, NPAN = HD / 64;
-    constexpr uint32_t NSB = PREC ? C::NSB_LO : 3;
+    constexpr uint32_t NSB = C::NSB, FOLD = C::FOLD;
     using Sched = PagedSched<BN, BM>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -133,9 +173,6 @@ __global__ void __launch_bounds__(kTThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->u_empty[ui % NU]);
     };
-    // keys the tile's last row sees
-    auto unit_keys = [&](const PagedUnit& u) -> int32_t { return Sched::keys(p, PagedReq{u.tok0, u.n, u.len}, u.j); };
-
     if (warp == 11) {
         // ================= schedule =================
         uint32_t ui = 0;
@@ -170,7 +207,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
         bool ok = true;
         PagedUnit u;
         for (uint32_t ui = 0; ok && get_unit(ui, u); ++ui) {
-            const uint32_t kend = static_cast<uint32_t>(unit_keys(u));
+            const uint32_t kend = static_cast<uint32_t>(u.keys);
             auto row_of = [&](uint32_t b) -> int32_t {
                 const uint32_t key = b * BN + i_pg * box;
                 if (!mine || key >= kend) return -1;
@@ -222,7 +259,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 put_unit(ui);
                 continue;
             }
-            const int32_t kend = unit_keys(u);
+            const int32_t kend = u.keys;
             ok = warp_wait_bounded(&bars->q_full, qph, status, ST_PAGED_TIMEOUT, abort_flag);
             qph ^= 1u;
             tc_fence_after();
@@ -240,11 +277,15 @@ __global__ void __launch_bounds__(kTThreads, 1)
                         const uint64_t b = dk + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4);
                         umma_f16(d, a, b, IDESC_QK, kk > 0 ? 1u : 0u);
                     }
-                    if constexpr (PREC) {   // + Q_lo K^T, A from TMEM
+                    if constexpr (PREC) {   // + Q_lo K^T
 #pragma unroll
                         for (int kk = 0; kk < HD / 16; ++kk) {
                             const uint64_t b = dk + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4);
-                            umma_f16_ts(d, tmem + C::qlo_col(kk), b, IDESC_QK, 1u);
+                            if constexpr (C::LO_SMEM)
+                                umma_f16(d, dq0 + ((C::OFF_QLO - C::OFF_Q + (kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4), b,
+                                         IDESC_QK, 1u);
+                            else
+                                umma_f16_ts(d, tmem + C::COL_QLO + 8 * kk, b, IDESC_QK, 1u);
                         }
                     }
                     umma_commit(&bars->s_full[s_sb]);
@@ -279,6 +320,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 if (lane == 0) {
                     const uint32_t pcol = tmem + C::COL_S + pv_sb * BN;
                     const uint64_t dv = dv0 + ((vs * C::KV_BYTES) >> 4);
+                    const bool fresh = PREC ? jj % FOLD == 0 : jj == 0;   // PREC: the sum so far has been folded
 #pragma unroll
                     for (int plane = 0; plane < (PREC ? 2 : 1); ++plane)
 #pragma unroll
@@ -286,7 +328,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                             if (kk < steps)
                                 umma_f16_ts(tmem + C::COL_O, pcol + 32 * (kk >> 1) + 16 * plane + 8 * (kk & 1),
                                             dv + ((kk * 2 * NPAN * 1024) >> 4), IDESC_PV,
-                                            (jj > 0 || plane > 0 || kk > 0) ? 1u : 0u);
+                                            (!fresh || plane > 0 || kk > 0) ? 1u : 0u);
                     umma_commit(&bars->v_empty[vs]);
                     umma_commit(&bars->pv_done[pv_sb]);
                 }
@@ -323,6 +365,8 @@ __global__ void __launch_bounds__(kTThreads, 1)
         const uint32_t trow = tmem + (static_cast<uint32_t>(qd * 32) << 16);
         uint32_t sb = 0, sph = 0, pb = 0, pph = 0;       // S buffer of this block / of the last one, and parities
         uint32_t oph = 0;
+        uint8_t* stg = smem + C::OFF_STG + warp * 2048;
+        float* s_up = reinterpret_cast<float*>(smem + C::OFF_UP);
         // Waits' results are ANDed over the warps that meet at the next barrier, so all of them leave together.
         for (uint32_t ui = 0;; ++ui) {
             PagedUnit u;
@@ -330,95 +374,169 @@ __global__ void __launch_bounds__(kTThreads, 1)
             if (!named_bar_and(5, 256, got)) break;      // the end, or a wait that gave up
             const uint32_t nb = u.kb1 - u.kb0;
             const uint32_t row0 = u.j * BM, rows = min(static_cast<uint32_t>(BM), static_cast<uint32_t>(u.n) * p.group - row0);
-            const bool live = static_cast<uint32_t>(r) < rows;
             const bool work = static_cast<uint32_t>(qd * 32) < rows;      // this warp has a live row
+            // this thread's row (padding rows: the last one again) and the column of its head
             const uint32_t f = row0 + min(static_cast<uint32_t>(r), rows - 1);
-            const uint32_t tk = f / p.group;
-            const size_t tok = u.tok0 + static_cast<size_t>(tk);
-            const size_t col0 = static_cast<size_t>(u.g * p.group + f % p.group) * HD + h * (HD / 2);
+            const uint32_t tk = div_group(p, f);
+            const uint32_t hcol = (u.g * p.group + f - tk * p.group) * HD;
             const int32_t qpos = u.len - u.n + static_cast<int32_t>(tk);   // last key this row sees
-            const int32_t qpos_min = u.len - u.n + static_cast<int32_t>(row0 / p.group);
-            auto write_out = [&](int c, const float (&x)[32]) {             // columns [c, c + 32) of this half
-                if (!live) return;
-                float y[32];
+            const int32_t qpos_min = u.len - u.n + static_cast<int32_t>(div_group(p, row0));
+            // Columns [c, c + 32) of this half's rows, a row per lane, gated and rounded, out through the warp's
+            // staging.  All lanes.
+            auto write_out = [&](int c, const float (&x)[32]) {
+                constexpr int ES = PREC ? 4 : 2, CW = 64 / ES;             // columns of a 64-byte run
+                // lane: 16 bytes of rows lane / 4 + 8 i of the warp
+                size_t at[4];
+                bool in[4];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) y[i] = x[i];
-                if (p.gate) {
-                    const size_t gi = tok * p.gate_stride + col0 + c;
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float2 g = ld_act2(p.gate, gi + i, p.act);
-                        y[i] *= sigmoid_of(g.x);
-                        y[i + 1] *= sigmoid_of(g.y);
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    const int rr = i * 8 + (lane >> 2);
+                    at[i] = static_cast<size_t>(u.tok0) + __shfl_sync(0xffffffffu, tk, rr);
+                    in[i] = static_cast<uint32_t>(qd * 32 + rr) < rows;
                 }
-                const size_t oi = tok * p.out_stride + col0 + c;
-                if constexpr (PREC) {
-                    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.out) + oi);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) dst[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-                } else {
-                    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + oi);
+                for (int sub = 0; sub < 32 / CW; ++sub) {
+                    float y[CW];
+#pragma unroll
+                    for (int i = 0; i < CW; ++i) y[i] = x[sub * CW + i];
+                    size_t col[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        col[i] = __shfl_sync(0xffffffffu, hcol, i * 8 + (lane >> 2)) + static_cast<size_t>(h * (HD / 2) + c + sub * CW + (lane & 3) * (16 / ES));
                     uint32_t w[16];
+                    if (p.gate) {
+                        uint4 raw[4];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if (p.act == YATTN_ACT_F16) {
-                            w[i] = h2_bits(__floats2half2_rn(y[2 * i], y[2 * i + 1]));
+                        for (int i = 0; i < 4; ++i) {
+                            raw[i] = make_uint4(0u, 0u, 0u, 0u);
+                            if (in[i])
+                                raw[i] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const char*>(p.gate) + (at[i] * p.gate_stride + col[i]) * ES));
+                        }
+                        stage_in(stg, lane, raw, w);
+                        if constexpr (PREC) {
+#pragma unroll
+                            for (int i = 0; i < CW; ++i) y[i] *= sigmoid_of(__uint_as_float(w[i]));
                         } else {
-                            const __nv_bfloat162 b = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
-                            w[i] = *reinterpret_cast<const uint32_t*>(&b);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const float2 t = p.act == YATTN_ACT_F16
+                                                     ? h2f2(w[i])
+                                                     : make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+                                y[2 * i] *= sigmoid_of(t.x);
+                                y[2 * i + 1] *= sigmoid_of(t.y);
+                            }
                         }
                     }
+                    if constexpr (PREC) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) dst[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                        for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(y[i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            if (p.act == YATTN_ACT_F16) {
+                                w[i] = h2_bits(__floats2half2_rn(y[2 * i], y[2 * i + 1]));
+                            } else {
+                                const __nv_bfloat162 b = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
+                                w[i] = *reinterpret_cast<const uint32_t*>(&b);
+                            }
+                        }
+                    }
+                    uint4 raw[4];
+                    stage_out(stg, lane, w, raw);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (in[i])
+                            *reinterpret_cast<uint4*>(static_cast<char*>(p.out) + (at[i] * p.out_stride + col[i]) * ES) = raw[i];
                 }
             };
             if (nb == 0) {                               // no key to see
                 float z[32];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) z[i] = 0.f;
+                if (work) {
 #pragma unroll 1
-                for (int c = 0; c < HD / 2; c += 32) write_out(c, z);
+                    for (int c = 0; c < HD / 2; c += 32) write_out(c, z);
+                }
                 put_unit(ui);
                 continue;
             }
 
-            // ---- Q: this thread's half row, scaled by the row's power of two ----
+            // ---- Q, each row scaled by its power of two: hi to shared memory, lo (PREC) beside it or to TMEM ----
             float up = 1.f;
             bool ok = true;
-            {
-                constexpr int CH = HD / 2 < 64 ? HD / 2 : 64;             // columns in registers at a time
-                float x[CH];
-                const size_t qi = tok * p.q_stride + col0;
-                auto load = [&](int c) {
+            if constexpr (!PREC || C::LO_SMEM) {
+                // warp w fetches rows 16 w .. + 15, LPR lanes a row, 16 bytes a lane
+                constexpr int ES = PREC ? 4 : 2, EL = 16 / ES, LPR = HD / EL, RPI = 32 / LPR, NI = 16 / RPI;
+                uint4 raw[NI];
 #pragma unroll
-                    for (int i = 0; i < CH; ++i) x[i] = 0.f;
-                    if (!live) return;
+                for (int i = 0; i < NI; ++i) {
+                    const uint32_t row = warp * 16 + i * RPI + lane / LPR;
+                    const uint32_t fr = row0 + min(row, rows - 1), tr = div_group(p, fr);
+                    const size_t at = (static_cast<size_t>(u.tok0) + tr) * p.q_stride +
+                                      (u.g * p.group + fr - tr * p.group) * HD + (lane % LPR) * EL;
+                    raw[i] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + at * ES));
+                }
+#pragma unroll
+                for (int i = 0; i < NI; ++i) {
+                    const uint32_t row = warp * 16 + i * RPI + lane / LPR;
+                    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                    float x[EL], mx = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if constexpr (PREC) {
+                            x[k] = __uint_as_float(w[k]);
+                        } else {
+                            const float2 t = p.act == YATTN_ACT_F16
+                                                 ? h2f2(w[k])
+                                                 : make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+                            x[2 * k] = t.x;
+                            x[2 * k + 1] = t.y;
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < EL; ++k) mx = fmaxf(mx, fabsf(x[k]));
+#pragma unroll
+                    for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                    float down, rup;
+                    row_scale(mx, down, rup);
+                    if (lane % LPR == 0) s_up[row] = rup;
+                    uint32_t hi[EL / 2], lo[EL / 2];
+#pragma unroll
+                    for (int k = 0; k < EL / 2; ++k) {
+                        const float a = x[2 * k] * down, b = x[2 * k + 1] * down;
+                        const __half2 hv = __floats2half2_rn(a, b);
+                        hi[k] = h2_bits(hv);
+                        const float2 fv = __half22float2(hv);
+                        lo[k] = h2_bits(__floats2half2_rn(a - fv.x, b - fv.y));
+                    }
+                    uint8_t* dst = sQ + sw128_offset(row, (lane % LPR) * EL, BM);
                     if constexpr (PREC) {
-                        const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + qi + c);
-#pragma unroll
-                        for (int i = 0; i < CH / 4; ++i) {
-                            const float4 v = __ldg(src + i);
-                            x[4 * i] = v.x;
-                            x[4 * i + 1] = v.y;
-                            x[4 * i + 2] = v.z;
-                            x[4 * i + 3] = v.w;
-                        }
+                        *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+                        *reinterpret_cast<uint2*>(dst + (C::OFF_QLO - C::OFF_Q)) = make_uint2(lo[0], lo[1]);
                     } else {
-                        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + qi + c);
+                        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    }
+                }
+                fence_proxy_async_smem();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars->q_full);
+                named_bar_sync(5, 256);                                   // s_up of every row
+                up = s_up[r];
+            } else {
+                // head_dim 256, fp32: a row's half per lane, in two passes (its largest value, then the planes)
+                constexpr int CH = 64;                                    // columns in registers at a time
+                float x[CH];
+                const size_t qi = (static_cast<size_t>(u.tok0) + tk) * p.q_stride + hcol + h * (HD / 2);
+                auto load = [&](int c) {
+                    const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + qi + c);
 #pragma unroll
-                        for (int i = 0; i < CH / 8; ++i) {
-                            const uint4 v = __ldg(src + i);
-                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const float2 t = p.act == YATTN_ACT_F16
-                                                     ? h2f2(w[k])
-                                                     : make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
-                                x[8 * i + 2 * k] = t.x;
-                                x[8 * i + 2 * k + 1] = t.y;
-                            }
-                        }
+                    for (int i = 0; i < CH / 4; ++i) {
+                        const float4 v = __ldg(src + i);
+                        x[4 * i] = v.x;
+                        x[4 * i + 1] = v.y;
+                        x[4 * i + 2] = v.z;
+                        x[4 * i + 3] = v.w;
                     }
                 };
                 float mx = 0.f;
@@ -453,15 +571,67 @@ __global__ void __launch_bounds__(kTThreads, 1)
                         for (int k = 0; k < 4; ++k)
                             *reinterpret_cast<uint4*>(sQ + sw128_offset(r, d0 + i + 8 * k, BM)) =
                                 make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
-                        if constexpr (PREC) tmem_st16(trow + C::qlo_col((d0 + i) / 16), lo);
+                        tmem_st16(trow + C::COL_QLO + (d0 + i) / 2, lo);
                     }
                 }
-                if constexpr (PREC) tmem_wait_st();
+                tmem_wait_st();
                 fence_proxy_async_smem();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars->q_full);
             }
+            // ---- O and (PREC) the folded sum, 32 columns of this half at a time ----
+            const uint32_t ocol = trow + C::COL_O + h * (HD / 2), fcol = trow + C::COL_F + h * (HD / 2);
+            const int quad0 = h * (HD / 8);              // this half's first column quad
+            auto quads = [&](uint32_t slot) {            // partials by column quads: a warp's accesses are whole lines
+                return reinterpret_cast<float4*>(p.part_o) + (static_cast<size_t>(slot) * (HD / 4) + quad0) * BM + r;
+            };
+            float4* const fsum = quads(2 * gridDim.x + blockIdx.x);
+            auto ld_fold = [&](int c, float (&x)[32]) {
+                if constexpr (C::FOLD_TMEM) {
+                    uint32_t rr[32];
+                    tmem_ld32(fcol + c, rr);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(rr[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float4 v = fsum[(c / 4 + i) * BM];
+                        x[4 * i] = v.x;
+                        x[4 * i + 1] = v.y;
+                        x[4 * i + 2] = v.z;
+                        x[4 * i + 3] = v.w;
+                    }
+                }
+            };
+            auto st_fold = [&](int c, const float (&x)[32]) {
+                if constexpr (C::FOLD_TMEM) {
+                    uint32_t rr[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) rr[i] = __float_as_uint(x[i]);
+                    tmem_st32(fcol + c, rr);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        fsum[(c / 4 + i) * BM] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                }
+            };
+            auto ld_o = [&](int c, float (&x)[32], bool folded) {           // the whole sum so far
+                uint32_t rr[32];
+                tmem_ld32(ocol + c, rr);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(rr[i]);
+                if constexpr (PREC) {
+                    if (folded) {
+                        float y[32];
+                        ld_fold(c, y);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[i] += y[i];
+                    }
+                }
+            };
             const float sl2 = p.scale_log2 * up;
             float m_run = -INFINITY, l_run = 0.f;        // log2 units; l_run: this half's columns
             for (uint32_t j = 0; j < nb; ++j) {
@@ -538,24 +708,39 @@ __global__ void __launch_bounds__(kTThreads, 1)
                     }
                     l_run = l_run * alpha + ((rs2[0].x + rs2[0].y) + (rs2[1].x + rs2[1].y));
                     m_run = m_use;
-                    // ---- O rescale (rare), this half's columns: the last block's PV must have finished.  Both
-                    // halves of the rows see the same `grow`. ----
-                    if (j >= 1 && __any_sync(0xffffffffu, grow)) {
+                    // ---- O rescale (rare) or fold (PREC), this half's columns: the last block's PV must have
+                    // finished.  Both halves of the rows see the same `grow`. ----
+                    const bool fold = PREC && j >= 1 && j % FOLD == 0;
+                    if (j >= 1 && (fold || __any_sync(0xffffffffu, grow))) {
                         const bool done = warp_wait_bounded(&bars->pv_done[pb], pph, status, ST_PAGED_TIMEOUT, abort_flag);
                         if (!named_bar_and(1 + qd, 64, done)) {
                             ok = false;
                             break;
                         }
                         tc_fence_after();
+                        const bool folded = PREC && j > FOLD;
 #pragma unroll 1
-                        for (int c = 0; c < HD / 64; ++c) {
-                            const uint32_t oc = trow + C::COL_O + h * (HD / 2) + c * 32;
-                            uint32_t rr[32];
-                            tmem_ld32(oc, rr);
-                            tmem_wait_ld();
+                        for (int c = 0; c < HD / 2; c += 32) {
+                            float x[32];
+                            ld_o(c, x, fold && folded);
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) rr[i] = __float_as_uint(__uint_as_float(rr[i]) * alpha);
-                            tmem_st32(oc, rr);
+                            for (int i = 0; i < 32; ++i) x[i] *= alpha;
+                            if (fold) {
+                                st_fold(c, x);
+                                continue;
+                            }
+                            uint32_t rr[32];
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) rr[i] = __float_as_uint(x[i]);
+                            tmem_st32(ocol + c, rr);
+                            if constexpr (PREC) {
+                                if (folded) {
+                                    ld_fold(c, x);
+#pragma unroll
+                                    for (int i = 0; i < 32; ++i) x[i] *= alpha;
+                                    st_fold(c, x);
+                                }
+                            }
                         }
                     }
                     tmem_wait_st();
@@ -579,40 +764,33 @@ __global__ void __launch_bounds__(kTThreads, 1)
             tc_fence_after();
             const float l_row = xl[r] + xl[BM + r];
             named_bar_sync(1 + qd, 64);                  // read before the next unit's Q maxima
-            const uint32_t ocol = trow + C::COL_O + h * (HD / 2);
+            const bool folded = PREC && nb > FOLD;
             if (u.n_pieces == 1) {
                 const float inv = l_row == 0.f ? 0.f : 1.0f / l_row;
+                if (work) {
 #pragma unroll 1
-                for (int c = 0; c < HD / 2; c += 32) {
-                    uint32_t rr[32];
-                    tmem_ld32(ocol + c, rr);
-                    tmem_wait_ld();
-                    float x[32];
+                    for (int c = 0; c < HD / 2; c += 32) {
+                        float x[32];
+                        ld_o(c, x, folded);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(rr[i]) * inv;
-                    write_out(c, x);
+                        for (int i = 0; i < 32; ++i) x[i] *= inv;
+                        write_out(c, x);
+                    }
                 }
                 tc_fence_before();
                 put_unit(ui);
                 continue;
             }
-            // ---- a piece: (m, l, o), o by column quads so that a warp's stores are whole lines ----
-            const int quad0 = h * (HD / 8);              // this half's first column quad
-            auto quads = [&](uint32_t slot) {
-                return reinterpret_cast<float4*>(p.part_o) + (static_cast<size_t>(slot) * (HD / 4) + quad0) * BM + r;
-            };
+            // ---- a piece: (m, l, o) ----
             if (h == 0) *reinterpret_cast<float2*>(&p.part_ml[(static_cast<size_t>(u.slot) * BM + r) * 2]) = make_float2(m_run, l_row);
-            float4* po = quads(u.slot);
+            if (work) {
+                float4* po = quads(u.slot);
 #pragma unroll 1
-            for (int c = 0; c < HD / 2; c += 32) {
-                uint32_t rr[32];
-                tmem_ld32(ocol + c, rr);
-                tmem_wait_ld();
-                if (live) {
+                for (int c = 0; c < HD / 2; c += 32) {
+                    float x[32];
+                    ld_o(c, x, folded);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        po[(c / 4 + i) * BM] = make_float4(__uint_as_float(rr[4 * i]), __uint_as_float(rr[4 * i + 1]),
-                                                           __uint_as_float(rr[4 * i + 2]), __uint_as_float(rr[4 * i + 3]));
+                    for (int i = 0; i < 8; ++i) po[(c / 4 + i) * BM] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
                 }
             }
             tc_fence_before();
@@ -621,14 +799,16 @@ __global__ void __launch_bounds__(kTThreads, 1)
             if (threadIdx.x == 0)
                 bars->last_flag = atomicInc(&p.counters[u.c_first], u.n_pieces - 1) == u.n_pieces - 1;
             named_bar_sync(5, 256);
-            if (bars->last_flag && live) {               // the last piece to arrive merges them, in piece order
+            if (bars->last_flag && work) {               // the last piece to arrive merges them, in piece order
                 __threadfence();
                 auto ml_of = [&](uint32_t i) {
                     return __ldcg(reinterpret_cast<const float2*>(
                         &p.part_ml[(static_cast<size_t>(piece_slot(u.c_first, i)) * BM + r) * 2]));
                 };
                 float M = -INFINITY, l = 0.f;
+#pragma unroll 4
                 for (uint32_t i = 0; i < u.n_pieces; ++i) M = fmaxf(M, ml_of(i).x);
+#pragma unroll 4
                 for (uint32_t i = 0; i < u.n_pieces; ++i) {
                     const float2 ml = ml_of(i);
                     l += (ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - M)) * ml.y;
@@ -639,20 +819,26 @@ __global__ void __launch_bounds__(kTThreads, 1)
                     float x[32];
 #pragma unroll
                     for (int i = 0; i < 32; ++i) x[i] = 0.f;
-#pragma unroll 2
-                    for (uint32_t i = 0; i < u.n_pieces; ++i) {
-                        const float4* src = quads(piece_slot(u.c_first, i)) + (c / 4) * BM;
-                        float4 o[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) o[k] = __ldcg(src + k * BM);
-                        const float mi = ml_of(i).x;
-                        const float w = mi == -INFINITY ? 0.f : ex2_approx(mi - M) * inv;
+#pragma unroll 1
+                    for (uint32_t i = 0; i < u.n_pieces; i += 2) {          // two pieces' loads in flight
+                        const uint32_t i1 = min(i + 1, u.n_pieces - 1);
+                        const float4* s0 = quads(piece_slot(u.c_first, i)) + (c / 4) * BM;
+                        const float4* s1 = quads(piece_slot(u.c_first, i1)) + (c / 4) * BM;
+                        const float m0 = ml_of(i).x, m1 = ml_of(i1).x;
+                        float4 o0[8], o1[8];
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
-                            x[4 * k] += w * o[k].x;
-                            x[4 * k + 1] += w * o[k].y;
-                            x[4 * k + 2] += w * o[k].z;
-                            x[4 * k + 3] += w * o[k].w;
+                            o0[k] = __ldcg(s0 + k * BM);
+                            o1[k] = __ldcg(s1 + k * BM);
+                        }
+                        const float w0 = m0 == -INFINITY ? 0.f : ex2_approx(m0 - M) * inv;
+                        const float w1 = m1 == -INFINITY || i1 == i ? 0.f : ex2_approx(m1 - M) * inv;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            x[4 * k] += w0 * o0[k].x + w1 * o1[k].x;
+                            x[4 * k + 1] += w0 * o0[k].y + w1 * o1[k].y;
+                            x[4 * k + 2] += w0 * o0[k].z + w1 * o1[k].z;
+                            x[4 * k + 3] += w0 * o0[k].w + w1 * o1[k].w;
                         }
                     }
                     write_out(c, x);
@@ -670,7 +856,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
 template <int HD, bool PREC>
 int launch(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, uint32_t ctas, cudaStream_t st,
            char* err, size_t errlen) {
-    using C = TCfg<HD>;
+    using C = TCfg<HD, PREC>;
     static bool attr_done[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
