@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = bars->tmem_base;
+    const uint32_t tmem = warp_uniform(bars->tmem_base);
 
     // Unit ui of the list, for one warp: waits for its descriptor.  false: the list has ended (or a wait gave up).
     auto get_unit = [&](uint32_t ui, PagedUnit& u) -> bool {
@@ -268,9 +268,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
             auto do_s = [&]() -> bool {
                 if (!warp_wait_bounded(&bars->k_full[ks], kph, status, ST_PAGED_TIMEOUT, abort_flag)) return false;
                 tc_fence_after();
-                if (lane == 0) {
-                    const uint64_t dk = dk0 + ((ks * C::KV_BYTES) >> 4);
-                    const uint32_t d = tmem + C::COL_S + s_sb * BN;
+                const uint64_t dk = dk0 + warp_uniform((ks * C::KV_BYTES) >> 4);
+                const uint32_t d = tmem + C::COL_S + warp_uniform(s_sb * BN);
+                if (elect_one()) {
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; ++kk) {
                         const uint64_t a = dq0 + (((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4);
@@ -317,9 +317,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
                     fence_proxy_async_smem();
                     __syncwarp();
                 }
-                if (lane == 0) {
-                    const uint32_t pcol = tmem + C::COL_S + pv_sb * BN;
-                    const uint64_t dv = dv0 + ((vs * C::KV_BYTES) >> 4);
+                const uint32_t pcol = tmem + C::COL_S + warp_uniform(pv_sb * BN);
+                const uint64_t dv = dv0 + warp_uniform((vs * C::KV_BYTES) >> 4);
+                if (elect_one()) {
                     const bool fresh = PREC ? jj % FOLD == 0 : jj == 0;   // PREC: the sum so far has been folded
 #pragma unroll
                     for (int plane = 0; plane < (PREC ? 2 : 1); ++plane)
@@ -348,11 +348,11 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 ok = do_pv(jj);
                 if (ok && jj + NSB < nb) ok = do_s();
             }
-            if (ok && lane == 0) umma_commit(&bars->o_done);
+            if (ok && elect_one()) umma_commit(&bars->o_done);
             put_unit(ui);
         }
         // every MMA issued so far completes before TMEM is freed
-        if (lane == 0) {
+        if (elect_one()) {
             umma_commit(&bars->mma_drain);
             volatile int dummy = 0;
             mbar_wait_bounded(&bars->mma_drain, 0, status, ST_PAGED_TIMEOUT, &dummy);

@@ -151,6 +151,22 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
         : "memory");
 }
 
+// True in one lane of the (converged) warp.  A branch on elect.sync is known to run one lane: the operands of the
+// products in it stay in uniform registers (where the instruction reads them) if warp_uniform() made them so.  In a
+// branch on the lane number each 128x128x16 product took 95 to 104 cycles to issue instead of 68 to 75, of which the
+// tensor core needs 64.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r != 0;
+}
+// Lane 0's value in every lane.
+__device__ __forceinline__ uint32_t warp_uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 // Arrives once on the mbarrier when every MMA this thread issued so far is done.
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
