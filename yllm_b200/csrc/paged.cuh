@@ -236,6 +236,7 @@ template <int BN, int ROWS> struct PagedSched {
     // The first CTA whose share ends at x or behind it.
     __device__ __forceinline__ uint32_t ends_at(long long x) const {
         uint32_t c = 0;
+#pragma unroll 1
         for (uint32_t k = 0; k < n_active; k += 32)
             c += __popc(__ballot_sync(0xffffffffu, k + lane < n_active && border(k + lane + 1) < x));
         return c;
@@ -255,7 +256,7 @@ template <int BN, int ROWS> struct PagedSched {
             sum += w;
             units += tiles(p, q);
         }
-#pragma unroll
+#pragma unroll 1                                  // (rolled: this runs once, and its instructions are fetched cold)
         for (int o = 16; o > 0; o >>= 1) {
             sum += __shfl_xor_sync(0xffffffffu, sum, o);
             units += __shfl_xor_sync(0xffffffffu, units, o);
@@ -278,7 +279,7 @@ template <int BN, int ROWS> struct PagedSched {
         bool found = false;
         auto look = [&](uint32_t chunk, long long w) {
             long long s = w;
-#pragma unroll
+#pragma unroll 1
             for (int o = 1; o < 32; o <<= 1) {
                 const long long u = __shfl_up_sync(0xffffffffu, s, o);
                 if (lane >= o) s += u;
@@ -293,6 +294,7 @@ template <int BN, int ROWS> struct PagedSched {
                 carry += __shfl_sync(0xffffffffu, s, 31);
             }
         };
+#pragma unroll 1
         for (uint32_t chunk = 0; !found && chunk < p.n_seqs; chunk += 32)
             look(chunk, chunk == 0 ? first : chunk + lane < p.n_seqs ? weight(p, paged_req(p, chunk + lane)) : 0);
         // the tile of r that holds y: before() grows with t

@@ -76,6 +76,7 @@ template <int KST, int VST> struct TBars {
     int abort_flag, last_flag;
 };
 
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 
 // A warp's 32 rows of 64 bytes through 2 KB of shared memory, 16-byte chunk c of row r at c ^ (r / 2 & 3): from
@@ -189,6 +190,21 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 mbar_arrive(&bars->u_full[ui % NU]);
             }
             if (!ok || !more) break;
+            // its rows of q and of the gate on their way to L2, a few units ahead of their use
+            const uint32_t row0 = u.j * BM, rows = min(static_cast<uint32_t>(BM), static_cast<uint32_t>(u.n) * p.group - row0);
+#pragma unroll 1
+            for (uint32_t i = lane; i < rows; i += 32) {
+                const uint32_t tk = div_group(p, row0 + i);
+                const size_t tok = static_cast<size_t>(u.tok0) + tk, col = (u.g * p.group + row0 + i - tk * p.group) * HD;
+                constexpr int ES = PREC ? 4 : 2;
+                const char* q = static_cast<const char*>(p.q) + (tok * p.q_stride + col) * ES;
+                const char* gt = static_cast<const char*>(p.gate) + (tok * p.gate_stride + col) * ES;
+#pragma unroll 1
+                for (int c = 0; c < HD * ES; c += 128) {
+                    prefetch_l2(q + c);
+                    if (p.gate) prefetch_l2(gt + c);
+                }
+            }
             ++ui;
         }
     } else if (warp == 8 || warp == 10) {
@@ -474,8 +490,16 @@ __global__ void __launch_bounds__(kTThreads, 1)
                     const uint32_t fr = row0 + min(row, rows - 1), tr = div_group(p, fr);
                     const size_t at = (static_cast<size_t>(u.tok0) + tr) * p.q_stride +
                                       (u.g * p.group + fr - tr * p.group) * HD + (lane % LPR) * EL;
-                    raw[i] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + at * ES));
+                    raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + at * ES));
                 }
+                if (!PREC && p.act == YATTN_ACT_F16) {       // fp16 as it is
+#pragma unroll
+                    for (int i = 0; i < NI; ++i) {
+                        const uint32_t row = warp * 16 + i * RPI + lane / LPR;
+                        if (lane % LPR == 0) s_up[row] = 1.f;
+                        *reinterpret_cast<uint4*>(sQ + sw128_offset(row, (lane % LPR) * EL, BM)) = raw[i];
+                    }
+                } else {
 #pragma unroll
                 for (int i = 0; i < NI; ++i) {
                     const uint32_t row = warp * 16 + i * RPI + lane / LPR;
@@ -516,6 +540,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                     } else {
                         *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     }
+                }
                 }
                 fence_proxy_async_smem();
                 tc_fence_before();
