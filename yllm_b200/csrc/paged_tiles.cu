@@ -26,6 +26,7 @@
 #include "tcgen05.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace yattn {
 namespace {
@@ -33,6 +34,7 @@ namespace {
 constexpr int BM = static_cast<int>(kPagedTileRows);
 constexpr int kTThreads = 384;
 constexpr int NU = 4;                    // unit descriptors in flight
+constexpr int kRegsSoftmax = 200, kRegsRest = 104;   // registers per thread after the split: 256 and 128 threads
 // P's factor: m may be stale by 8 binades, and fp16 ends below 2^16
 constexpr float kPUp = 7.f;
 
@@ -112,10 +114,11 @@ __device__ __forceinline__ void stage_out(uint8_t* stg, int lane, const uint32_t
     __syncwarp();
 }
 
-template <int HD, bool PREC>
+template <int HD, int ACT>
 __global__ void __launch_bounds__(kTThreads, 1)
     k_paged_tiles(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const __grid_constant__ PagedParams p) {
+    constexpr bool PREC = ACT == YATTN_ACT_F32;
     using C = TCfg<HD, PREC>;
     constexpr int BN = C::BN, HB = BN / 2, KST = C::KST, VST = C::VST, NPAN = HD / 64;
     constexpr uint32_t NSB = C::NSB, FOLD = C::FOLD;
@@ -174,6 +177,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars->u_empty[ui % NU]);
     };
+    // registers move to the softmax warps (the launcher checks the sum against the launch's)
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
     if (warp == 11) {
         // ================= schedule =================
         uint32_t ui = 0;
@@ -255,7 +261,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
         volatile int dummy = 0;
         for (uint32_t b = issued > depth ? issued - depth : 0; b < issued; ++b)
             mbar_wait_bounded(&full[b % depth], (b / depth) & 1u, status, ST_PAGED_TIMEOUT, &dummy);
-    } else if (warp == 9) {
+    } else {
         // ================= MMA =================
         constexpr uint32_t IDESC_QK = idesc_f16(BM, BN, 0);
         constexpr uint32_t IDESC_PV = idesc_f16(BM, HD, 1);
@@ -374,7 +380,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
             mbar_wait_bounded(&bars->mma_drain, 0, status, ST_PAGED_TIMEOUT, &dummy);
         }
         __syncwarp();
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         // ================= softmax warps 0-7 =================
         const int qd = warp & 3, h = warp >> 2;          // TMEM lane quadrant, half of each block's columns
         const int r = qd * 32 + lane;                    // row of the tile
@@ -398,36 +406,38 @@ __global__ void __launch_bounds__(kTThreads, 1)
             const int32_t qpos = u.len - u.n + static_cast<int32_t>(tk);   // last key this row sees
             const int32_t qpos_min = u.len - u.n + static_cast<int32_t>(div_group(p, row0));
             // Columns [c, c + 32) of this half's rows, a row per lane, gated and rounded, out through the warp's
-            // staging.  All lanes.
-            auto write_out = [&](int c, const float (&x)[32]) {
-                constexpr int ES = PREC ? 4 : 2, CW = 64 / ES;             // columns of a 64-byte run
-                // lane: 16 bytes of rows lane / 4 + 8 i of the warp
-                size_t at[4];
-                bool in[4];
+            // staging; g: their gate values from ld_gate(), in the staging's order.  All lanes.
+            constexpr int ES = PREC ? 4 : 2, CW = 64 / ES, SUBS = 32 / CW;   // columns of a 64-byte run, runs
+            // lane: 16 bytes of rows lane / 4 + 8 i of the warp
+            auto run_at = [&](int c, int i, size_t& token, size_t& col) -> bool {
+                const int rr = i * 8 + (lane >> 2);
+                token = static_cast<size_t>(u.tok0) + __shfl_sync(0xffffffffu, tk, rr);
+                col = __shfl_sync(0xffffffffu, hcol, rr) + static_cast<size_t>(h * (HD / 2) + c + (lane & 3) * (16 / ES));
+                return static_cast<uint32_t>(qd * 32 + rr) < rows;
+            };
+            auto ld_gate = [&](int c, uint4 (&g)[SUBS * 4]) {
+                if (!p.gate) return;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int rr = i * 8 + (lane >> 2);
-                    at[i] = static_cast<size_t>(u.tok0) + __shfl_sync(0xffffffffu, tk, rr);
-                    in[i] = static_cast<uint32_t>(qd * 32 + rr) < rows;
-                }
+                    size_t token, col;
+                    const bool in = run_at(c, i, token, col);
 #pragma unroll
-                for (int sub = 0; sub < 32 / CW; ++sub) {
+                    for (int sub = 0; sub < SUBS; ++sub) {
+                        g[sub * 4 + i] = make_uint4(0u, 0u, 0u, 0u);
+                        if (in)
+                            g[sub * 4 + i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(p.gate) + (token * p.gate_stride + col + sub * CW) * ES));
+                    }
+                }
+            };
+            auto write_out = [&](int c, const float (&x)[32], const uint4 (&g)[SUBS * 4]) {
+#pragma unroll
+                for (int sub = 0; sub < SUBS; ++sub) {
                     float y[CW];
 #pragma unroll
                     for (int i = 0; i < CW; ++i) y[i] = x[sub * CW + i];
-                    size_t col[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        col[i] = __shfl_sync(0xffffffffu, hcol, i * 8 + (lane >> 2)) + static_cast<size_t>(h * (HD / 2) + c + sub * CW + (lane & 3) * (16 / ES));
                     uint32_t w[16];
                     if (p.gate) {
-                        uint4 raw[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            raw[i] = make_uint4(0u, 0u, 0u, 0u);
-                            if (in[i])
-                                raw[i] = __ldcs(reinterpret_cast<const uint4*>(static_cast<const char*>(p.gate) + (at[i] * p.gate_stride + col[i]) * ES));
-                        }
+                        const uint4 raw[4] = {g[sub * 4], g[sub * 4 + 1], g[sub * 4 + 2], g[sub * 4 + 3]};
                         stage_in(stg, lane, raw, w);
                         if constexpr (PREC) {
 #pragma unroll
@@ -435,7 +445,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                         } else {
 #pragma unroll
                             for (int i = 0; i < 16; ++i) {
-                                const float2 t = p.act == YATTN_ACT_F16
+                                const float2 t = ACT == YATTN_ACT_F16
                                                      ? h2f2(w[i])
                                                      : make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
                                 y[2 * i] *= sigmoid_of(t.x);
@@ -449,7 +459,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            if (p.act == YATTN_ACT_F16) {
+                            if (ACT == YATTN_ACT_F16) {
                                 w[i] = h2_bits(__floats2half2_rn(y[2 * i], y[2 * i + 1]));
                             } else {
                                 const __nv_bfloat162 b = __floats2bfloat162_rn(y[2 * i], y[2 * i + 1]);
@@ -460,26 +470,72 @@ __global__ void __launch_bounds__(kTThreads, 1)
                     uint4 raw[4];
                     stage_out(stg, lane, w, raw);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (in[i])
-                            *reinterpret_cast<uint4*>(static_cast<char*>(p.out) + (at[i] * p.out_stride + col[i]) * ES) = raw[i];
+                    for (int i = 0; i < 4; ++i) {
+                        size_t token, col;
+                        if (run_at(c + sub * CW, i, token, col))
+                            *reinterpret_cast<uint4*>(static_cast<char*>(p.out) + (token * p.out_stride + col) * ES) = raw[i];
+                    }
                 }
             };
-            if (nb == 0) {                               // no key to see
-                float z[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i) z[i] = 0.f;
-                if (work) {
-#pragma unroll 1
-                    for (int c = 0; c < HD / 2; c += 32) write_out(c, z);
-                }
-                put_unit(ui);
-                continue;
-            }
-
-            // ---- Q, each row scaled by its power of two: hi to shared memory, lo (PREC) beside it or to TMEM ----
-            float up = 1.f;
+            const bool folded = PREC && nb > FOLD;
+            float m_run = -INFINITY, l_run = 0.f, l_row = 0.f;   // log2 units; l_run: this half's columns
+            uint4 g[SUBS * 4];                           // the gate of the next 32 columns, a step ahead
             bool ok = true;
+            // ---- O and (PREC) the folded sum, 32 columns of this half at a time ----
+            const uint32_t ocol = trow + C::COL_O + h * (HD / 2), fcol = trow + C::COL_F + h * (HD / 2);
+            const int quad0 = h * (HD / 8);              // this half's first column quad
+            auto quads = [&](uint32_t slot) {            // partials by column quads: a warp's accesses are whole lines
+                return reinterpret_cast<float4*>(p.part_o) + (static_cast<size_t>(slot) * (HD / 4) + quad0) * BM + r;
+            };
+            float4* const fsum = quads(2 * gridDim.x + blockIdx.x);
+            auto ld_fold = [&](int c, float (&x)[32]) {
+                if constexpr (C::FOLD_TMEM) {
+                    uint32_t rr[32];
+                    tmem_ld32(fcol + c, rr);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(rr[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float4 v = fsum[(c / 4 + i) * BM];
+                        x[4 * i] = v.x;
+                        x[4 * i + 1] = v.y;
+                        x[4 * i + 2] = v.z;
+                        x[4 * i + 3] = v.w;
+                    }
+                }
+            };
+            auto st_fold = [&](int c, const float (&x)[32]) {
+                if constexpr (C::FOLD_TMEM) {
+                    uint32_t rr[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) rr[i] = __float_as_uint(x[i]);
+                    tmem_st32(fcol + c, rr);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        fsum[(c / 4 + i) * BM] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                }
+            };
+            auto ld_o = [&](int c, float (&x)[32], bool folded) {           // the whole sum so far
+                uint32_t rr[32];
+                tmem_ld32(ocol + c, rr);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(rr[i]);
+                if constexpr (PREC) {
+                    if (folded) {
+                        float y[32];
+                        ld_fold(c, y);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[i] += y[i];
+                    }
+                }
+            };
+            if (nb > 0) {
+            float up = 1.f;
+            // ---- Q, each row scaled by its power of two: hi to shared memory, lo (PREC) beside it or to TMEM ----
             if constexpr (!PREC || C::LO_SMEM) {
                 // warp w fetches rows 16 w .. + 15, LPR lanes a row, 16 bytes a lane
                 constexpr int ES = PREC ? 4 : 2, EL = 16 / ES, LPR = HD / EL, RPI = 32 / LPR, NI = 16 / RPI;
@@ -492,7 +548,31 @@ __global__ void __launch_bounds__(kTThreads, 1)
                                       (u.g * p.group + fr - tr * p.group) * HD + (lane % LPR) * EL;
                     raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + at * ES));
                 }
-                if (!PREC && p.act == YATTN_ACT_F16) {       // fp16 as it is
+                // fp16 goes as it is; bf16 too where fp16 can hold this warp's rows (below 2^15; what falls under fp16's
+                // subnormals is off by 2^-25, far below the output's rounding), else scaled as fp32 is
+                bool plain = ACT == YATTN_ACT_F16;
+                if constexpr (ACT == YATTN_ACT_BF16) {
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int i = 0; i < NI; ++i)
+                        top = max(top, max(max(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu), max(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu)));
+                    uint32_t low = 0;
+#pragma unroll
+                    for (int i = 0; i < NI; ++i)
+                        low = max(low, max(max(raw[i].x & 0x7fffu, raw[i].y & 0x7fffu), max(raw[i].z & 0x7fffu, raw[i].w & 0x7fffu)));
+                    plain = __all_sync(0xffffffffu, (top >> 16) < 0x4700u && low < 0x4700u);
+                    if (plain) {
+#pragma unroll
+                        for (int i = 0; i < NI; ++i) {
+                            uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                w[k] = h2_bits(__floats2half2_rn(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u)));
+                            raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                }
+                if (plain) {
 #pragma unroll
                     for (int i = 0; i < NI; ++i) {
                         const uint32_t row = warp * 16 + i * RPI + lane / LPR;
@@ -510,7 +590,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                         if constexpr (PREC) {
                             x[k] = __uint_as_float(w[k]);
                         } else {
-                            const float2 t = p.act == YATTN_ACT_F16
+                            const float2 t = ACT == YATTN_ACT_F16
                                                  ? h2f2(w[k])
                                                  : make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
                             x[2 * k] = t.x;
@@ -519,8 +599,12 @@ __global__ void __launch_bounds__(kTThreads, 1)
                     }
 #pragma unroll
                     for (int k = 0; k < EL; ++k) mx = fmaxf(mx, fabsf(x[k]));
+                    if constexpr (LPR == 32) {               // (magnitudes order as their bits)
+                        mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
+                    } else {
 #pragma unroll
-                    for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                    }
                     float down, rup;
                     row_scale(mx, down, rup);
                     if (lane % LPR == 0) s_up[row] = rup;
@@ -605,60 +689,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars->q_full);
             }
-            // ---- O and (PREC) the folded sum, 32 columns of this half at a time ----
-            const uint32_t ocol = trow + C::COL_O + h * (HD / 2), fcol = trow + C::COL_F + h * (HD / 2);
-            const int quad0 = h * (HD / 8);              // this half's first column quad
-            auto quads = [&](uint32_t slot) {            // partials by column quads: a warp's accesses are whole lines
-                return reinterpret_cast<float4*>(p.part_o) + (static_cast<size_t>(slot) * (HD / 4) + quad0) * BM + r;
-            };
-            float4* const fsum = quads(2 * gridDim.x + blockIdx.x);
-            auto ld_fold = [&](int c, float (&x)[32]) {
-                if constexpr (C::FOLD_TMEM) {
-                    uint32_t rr[32];
-                    tmem_ld32(fcol + c, rr);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(rr[i]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float4 v = fsum[(c / 4 + i) * BM];
-                        x[4 * i] = v.x;
-                        x[4 * i + 1] = v.y;
-                        x[4 * i + 2] = v.z;
-                        x[4 * i + 3] = v.w;
-                    }
-                }
-            };
-            auto st_fold = [&](int c, const float (&x)[32]) {
-                if constexpr (C::FOLD_TMEM) {
-                    uint32_t rr[32];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) rr[i] = __float_as_uint(x[i]);
-                    tmem_st32(fcol + c, rr);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        fsum[(c / 4 + i) * BM] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-                }
-            };
-            auto ld_o = [&](int c, float (&x)[32], bool folded) {           // the whole sum so far
-                uint32_t rr[32];
-                tmem_ld32(ocol + c, rr);
-                tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(rr[i]);
-                if constexpr (PREC) {
-                    if (folded) {
-                        float y[32];
-                        ld_fold(c, y);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] += y[i];
-                    }
-                }
-            };
             const float sl2 = p.scale_log2 * up;
-            float m_run = -INFINITY, l_run = 0.f;        // log2 units; l_run: this half's columns
             for (uint32_t j = 0; j < nb; ++j) {
                 const bool have = warp_wait_bounded(&bars->s_full[sb], sph, status, ST_PAGED_TIMEOUT, abort_flag);
                 if (!work) {                             // no live row: P's lanes stay as they are, nothing reads them
@@ -780,6 +811,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                     sph ^= 1u;
                 }
             }
+            if (work) ld_gate(0, g);
             // ---- the unit's rows: the slot that block nb-1 did not use is free (both halves have read it) ----
             ok = ok && warp_wait_bounded(&bars->o_done, oph, status, ST_PAGED_TIMEOUT, abort_flag);
             oph ^= 1u;
@@ -787,88 +819,96 @@ __global__ void __launch_bounds__(kTThreads, 1)
             xl[h * BM + r] = l_run;
             if (!named_bar_and(5, 256, ok)) break;       // every softmax warp
             tc_fence_after();
-            const float l_row = xl[r] + xl[BM + r];
+            l_row = xl[r] + xl[BM + r];
             named_bar_sync(1 + qd, 64);                  // read before the next unit's Q maxima
-            const bool folded = PREC && nb > FOLD;
-            if (u.n_pieces == 1) {
-                const float inv = l_row == 0.f ? 0.f : 1.0f / l_row;
+            } else if (work) {                           // no key to see: zeros
+                ld_gate(0, g);
+            }
+            // ---- the unit's rows, or a piece's (m, l, o) and, of the last piece to arrive, the merged rows ----
+            bool write = work;
+            float M = -INFINITY, inv = l_row == 0.f ? 0.f : 1.0f / l_row;
+            auto ml_of = [&](uint32_t i) {
+                return __ldcg(reinterpret_cast<const float2*>(
+                    &p.part_ml[(static_cast<size_t>(piece_slot(u.c_first, i)) * BM + r) * 2]));
+            };
+            if (u.n_pieces > 1) {
+                if (h == 0)
+                    *reinterpret_cast<float2*>(&p.part_ml[(static_cast<size_t>(u.slot) * BM + r) * 2]) = make_float2(m_run, l_row);
                 if (work) {
+                    float4* po = quads(u.slot);
 #pragma unroll 1
                     for (int c = 0; c < HD / 2; c += 32) {
                         float x[32];
                         ld_o(c, x, folded);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] *= inv;
-                        write_out(c, x);
+                        for (int i = 0; i < 8; ++i)
+                            po[(c / 4 + i) * BM] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
                     }
                 }
-                tc_fence_before();
-                put_unit(ui);
-                continue;
+                __threadfence();
+                named_bar_sync(5, 256);
+                if (threadIdx.x == 0)
+                    bars->last_flag = atomicInc(&p.counters[u.c_first], u.n_pieces - 1) == u.n_pieces - 1;
+                named_bar_sync(5, 256);
+                write = bars->last_flag && work;
+                if (write) {
+                    __threadfence();
+                    float l = 0.f;
+#pragma unroll 4
+                    for (uint32_t i = 0; i < u.n_pieces; ++i) M = fmaxf(M, ml_of(i).x);
+#pragma unroll 4
+                    for (uint32_t i = 0; i < u.n_pieces; ++i) {
+                        const float2 ml = ml_of(i);
+                        l += (ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - M)) * ml.y;
+                    }
+                    inv = l == 0.f ? 0.f : 1.0f / l;
+                }
             }
-            // ---- a piece: (m, l, o) ----
-            if (h == 0) *reinterpret_cast<float2*>(&p.part_ml[(static_cast<size_t>(u.slot) * BM + r) * 2]) = make_float2(m_run, l_row);
-            if (work) {
-                float4* po = quads(u.slot);
+            if (write) {
 #pragma unroll 1
                 for (int c = 0; c < HD / 2; c += 32) {
+                    uint4 g_next[SUBS * 4];
+                    if (c + 32 < HD / 2) ld_gate(c + 32, g_next);
                     float x[32];
-                    ld_o(c, x, folded);
+                    if (u.n_pieces > 1) {                // in piece order
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) po[(c / 4 + i) * BM] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                        for (int i = 0; i < 32; ++i) x[i] = 0.f;
+#pragma unroll 1
+                        for (uint32_t i = 0; i < u.n_pieces; i += 2) {      // two pieces' loads in flight
+                            const uint32_t i1 = min(i + 1, u.n_pieces - 1);
+                            const float4* s0 = quads(piece_slot(u.c_first, i)) + (c / 4) * BM;
+                            const float4* s1 = quads(piece_slot(u.c_first, i1)) + (c / 4) * BM;
+                            const float m0 = ml_of(i).x, m1 = ml_of(i1).x;
+                            float4 o0[8], o1[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                o0[k] = __ldcg(s0 + k * BM);
+                                o1[k] = __ldcg(s1 + k * BM);
+                            }
+                            const float w0 = m0 == -INFINITY ? 0.f : ex2_approx(m0 - M) * inv;
+                            const float w1 = m1 == -INFINITY || i1 == i ? 0.f : ex2_approx(m1 - M) * inv;
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) {
+                                x[4 * k] += w0 * o0[k].x + w1 * o1[k].x;
+                                x[4 * k + 1] += w0 * o0[k].y + w1 * o1[k].y;
+                                x[4 * k + 2] += w0 * o0[k].z + w1 * o1[k].z;
+                                x[4 * k + 3] += w0 * o0[k].w + w1 * o1[k].w;
+                            }
+                        }
+                    } else if (nb > 0) {
+                        ld_o(c, x, folded);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[i] *= inv;
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[i] = 0.f;
+                    }
+                    write_out(c, x, g);
+#pragma unroll
+                    for (int i = 0; i < SUBS * 4; ++i) g[i] = g_next[i];
                 }
             }
             tc_fence_before();
-            __threadfence();
-            named_bar_sync(5, 256);
-            if (threadIdx.x == 0)
-                bars->last_flag = atomicInc(&p.counters[u.c_first], u.n_pieces - 1) == u.n_pieces - 1;
-            named_bar_sync(5, 256);
-            if (bars->last_flag && work) {               // the last piece to arrive merges them, in piece order
-                __threadfence();
-                auto ml_of = [&](uint32_t i) {
-                    return __ldcg(reinterpret_cast<const float2*>(
-                        &p.part_ml[(static_cast<size_t>(piece_slot(u.c_first, i)) * BM + r) * 2]));
-                };
-                float M = -INFINITY, l = 0.f;
-#pragma unroll 4
-                for (uint32_t i = 0; i < u.n_pieces; ++i) M = fmaxf(M, ml_of(i).x);
-#pragma unroll 4
-                for (uint32_t i = 0; i < u.n_pieces; ++i) {
-                    const float2 ml = ml_of(i);
-                    l += (ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - M)) * ml.y;
-                }
-                const float inv = l == 0.f ? 0.f : 1.0f / l;
-#pragma unroll 1
-                for (int c = 0; c < HD / 2; c += 32) {
-                    float x[32];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) x[i] = 0.f;
-#pragma unroll 1
-                    for (uint32_t i = 0; i < u.n_pieces; i += 2) {          // two pieces' loads in flight
-                        const uint32_t i1 = min(i + 1, u.n_pieces - 1);
-                        const float4* s0 = quads(piece_slot(u.c_first, i)) + (c / 4) * BM;
-                        const float4* s1 = quads(piece_slot(u.c_first, i1)) + (c / 4) * BM;
-                        const float m0 = ml_of(i).x, m1 = ml_of(i1).x;
-                        float4 o0[8], o1[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            o0[k] = __ldcg(s0 + k * BM);
-                            o1[k] = __ldcg(s1 + k * BM);
-                        }
-                        const float w0 = m0 == -INFINITY ? 0.f : ex2_approx(m0 - M) * inv;
-                        const float w1 = m1 == -INFINITY || i1 == i ? 0.f : ex2_approx(m1 - M) * inv;
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            x[4 * k] += w0 * o0[k].x + w1 * o1[k].x;
-                            x[4 * k + 1] += w0 * o0[k].y + w1 * o1[k].y;
-                            x[4 * k + 2] += w0 * o0[k].z + w1 * o1[k].z;
-                            x[4 * k + 3] += w0 * o0[k].w + w1 * o1[k].w;
-                        }
-                    }
-                    write_out(c, x);
-                }
-            }
             put_unit(ui);
         }
         tc_fence_before();
@@ -878,22 +918,29 @@ __global__ void __launch_bounds__(kTThreads, 1)
     if (warp == 0) tmem_dealloc(tmem, C::TMEM_COLS);
 }
 
-template <int HD, bool PREC>
+template <int HD, int ACT>
 int launch(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, uint32_t ctas, cudaStream_t st,
            char* err, size_t errlen) {
-    using C = TCfg<HD, PREC>;
+    using C = TCfg<HD, ACT == YATTN_ACT_F32>;
     static bool attr_done[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 0 && dev < 64 && !attr_done[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(k_paged_tiles<HD, PREC>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(k_paged_tiles<HD, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) {
             set_err(err, errlen, "attn_paged: smem attribute (%d bytes): %s", C::SMEM, cudaGetErrorString(e));
             return -1;
         }
+        // an increase past what the block was launched with would wait for ever
+        cudaFuncAttributes at{};
+        e = cudaFuncGetAttributes(&at, k_paged_tiles<HD, ACT>);
+        if (e != cudaSuccess || at.numRegs * kTThreads < 256 * kRegsSoftmax + 128 * kRegsRest) {
+            set_err(err, errlen, "attn_paged: built with %d registers a thread, too few for the register split", at.numRegs);
+            return -1;
+        }
         attr_done[dev] = true;
     }
-    k_paged_tiles<HD, PREC><<<ctas, kTThreads, C::SMEM, st>>>(mk, mv, p);
+    k_paged_tiles<HD, ACT><<<ctas, kTThreads, C::SMEM, st>>>(mk, mv, p);
     YATTN_CHECK_LAUNCH(err, errlen, "attn_paged");
     return 0;
 }
@@ -911,14 +958,18 @@ int paged_tiles(const PagedParams& pp, const uint16_t* kpool, const uint16_t* vp
         encode_page_map(&mv, vpool, kv_dim, n_rows, n_kv * hd, box, hd / 64, err, errlen))
         return -1;
     const uint32_t ctas = std::min<uint32_t>(static_cast<uint32_t>(dev_num_sms()), kPagedMaxPieces);
-    const bool prec = p.act == YATTN_ACT_F32;
+    auto run = [&](auto tag) -> int {
+        constexpr int HD = decltype(tag)::value;
+        switch (p.act) {
+            case YATTN_ACT_F32: return launch<HD, YATTN_ACT_F32>(p, mk, mv, ctas, st, err, errlen);
+            case YATTN_ACT_F16: return launch<HD, YATTN_ACT_F16>(p, mk, mv, ctas, st, err, errlen);
+            default: return launch<HD, YATTN_ACT_BF16>(p, mk, mv, ctas, st, err, errlen);
+        }
+    };
     switch (hd) {
-        case 64: return prec ? launch<64, true>(p, mk, mv, ctas, st, err, errlen)
-                             : launch<64, false>(p, mk, mv, ctas, st, err, errlen);
-        case 128: return prec ? launch<128, true>(p, mk, mv, ctas, st, err, errlen)
-                              : launch<128, false>(p, mk, mv, ctas, st, err, errlen);
-        default: return prec ? launch<256, true>(p, mk, mv, ctas, st, err, errlen)
-                             : launch<256, false>(p, mk, mv, ctas, st, err, errlen);
+        case 64: return run(std::integral_constant<int, 64>{});
+        case 128: return run(std::integral_constant<int, 128>{});
+        default: return run(std::integral_constant<int, 256>{});
     }
 }
 
