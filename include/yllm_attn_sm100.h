@@ -504,7 +504,8 @@ int yattn_sess_kv_load(uint16_t* kv_dev, uint32_t n_blocks, uint32_t kv_dim, uin
  * tables and slots are shared by the layers.  A serving step is one
  * yattn_page_step, then per layer yattn_rope_store_kv_paged and
  * yattn_attn_paged; all of them read lengths on the device, so a step can be
- * captured in a CUDA graph and replayed with other lengths. */
+ * captured in a CUDA graph and replayed with other lengths (the first call on
+ * a device, which allocates its status word, comes before any capture). */
 
 enum { YATTN_ACT_F32 = 0, YATTN_ACT_F16 = 1, YATTN_ACT_BF16 = 2 };   /* activation types */
 
@@ -574,7 +575,10 @@ int yattn_rope_store_kv_paged(void* q_out, uint32_t q_out_stride, const void* q,
  * A block table entry outside the pool reads as zero rows (device status 602);
  * a request whose offsets or lengths contradict the arguments, or which has
  * more than max_new tokens, is skipped, its rows of out not written (603).
- * head_dim 64/128/256, n_heads a multiple of n_kv_heads.
+ * Cache rows behind kv_len may hold anything.  A K or V row before it that is
+ * not finite reaches every token that sees it, and such a V row may also reach
+ * earlier tokens of its own chunk (0 * inf in a shared product).
+ * head_dim 64/128/256, n_heads a multiple of n_kv_heads; out overlaps nothing.
  * workspace: yattn_attn_paged_workspace_bytes, its first 4096 bytes zeroed once; a
  * call leaves them zero.  Calls that may overlap (other streams, graphs) need
  * a workspace each; after status 601 zero it again. */

@@ -247,3 +247,176 @@ def test_tiles_far_q(dev, act, scale):
     c = Case(dev, 8, 2, 128, 16, [50, 333], [20, 100], act=act, seed=4, q_scale=scale)
     c.run()
     c.check()
+
+
+# ------------------------------------------------------- what the calls refuse or report
+
+def test_bad_page_reads_as_zeros_and_is_reported(dev):
+    """A block table entry outside the pool: status 602, and the other requests are untouched by it."""
+    from yllm_b200 import attn
+    for new in ([1, 1], [40, 30]):
+        c = Case(dev, 8, 2, 64, 16, [100, 90], new, seed=6)
+        c.run()
+        torch.cuda.synchronize()
+        good = c.out.clone()
+        for entry in (-1, 1 << 20, 2 ** 31 - 1, c.kp.shape[0] // 16):
+            c.tables[0, 2] = entry
+            c.run()
+            torch.cuda.synchronize()
+            assert attn.device_status() == 602
+            assert torch.equal(c.out[new[0]:], good[new[0]:]) and bool(c.out[:new[0]].isfinite().all())
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [30, 1, 40]])
+@pytest.mark.parametrize("what", ["cu falls", "cu past the rows", "negative length", "length past the table", "max_new"])
+def test_contradicting_request_is_skipped_and_reported(dev, what, new):
+    from yllm_b200 import attn
+    c = Case(dev, 8, 2, 64, 16, [100, 90, 80], new, seed=7)
+    want, bar = c.want(max(new) * 4 <= ROWS)
+    kw = {}
+    skipped = 2
+    if what == "cu falls":
+        c.cu[3] = int(c.cu[2]) - 1
+    elif what == "cu past the rows":
+        c.cu[3] = c.q.shape[0] + 1
+    elif what == "negative length":
+        c.kv[2] = -5
+    elif what == "length past the table":
+        c.kv[2] = c.tables.shape[1] * 16 + 1
+    else:
+        if new[2] == 1:
+            return
+        kw["max_new"] = new[2] - 1     # still the tiles form
+    c.run(**kw)
+    torch.cuda.synchronize()
+    assert attn.device_status() == 603
+    a, b = sum(new[:skipped]), sum(new)
+    # (the others hold their bars; not bit for bit, as the work is divided anew without it)
+    assert bool(((c.out[:a, :512].double() - want[:a]).abs() <= bar[:a]).all()) and bool((c.out[a:b] == 3.0).all())
+    c.run(max_new=64)      # nothing of it lingers (its own lengths are still wrong for four of them)
+    attn.device_status()
+
+
+def test_rows_form_refuses_more_tokens_than_announced(dev):
+    from yllm_b200 import attn
+    c = Case(dev, 8, 2, 128, 16, [64, 200], [1, 3], seed=8)
+    c.run(max_new=1)
+    torch.cuda.synchronize()
+    assert attn.device_status() == 603 and bool((c.out[1:, :8 * 128] == 3.0).all())
+    c.run(max_new=3)
+    c.check(max_new=3)
+
+
+# ------------------------------------------------------------- streams, graphs, workspaces
+
+def test_two_streams_at_once(dev):
+    """Each stream has its own workspace: cut units of two calls in flight do not meet."""
+    cases = [Case(dev, 32, 8, 128, 16, [20000 + 777 * i], [1], seed=20 + i) for i in range(2)]
+    cases += [Case(dev, 8, 2, 128, 16, [9000 + 77 * i], [70], seed=30 + i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for c, s in zip(cases, streams):
+            c.run(stream=s)
+    torch.cuda.synchronize()
+    for c in cases:
+        c.check()
+
+
+def test_capture_and_replay_with_other_lengths(dev):
+    """Lengths and tables are read at replay: one graph serves growing requests.  Two graphs replayed at once on two
+    streams have workspaces of their own."""
+    from yllm_b200 import attn
+    H, KV, hd, page = 8, 2, 128, 16
+    big = [Case(dev, H, KV, hd, page, [6000, 50, 3000], [1, 1, 1], seed=40), Case(dev, H, KV, hd, page, [5000, 40, 300], [60, 1, 7], seed=41)]
+    for c in big:
+        c.run()
+    torch.cuda.synchronize()
+    graphs = []
+    for c in big:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.run()
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in big]
+    for cut in (0, 17, 2900):
+        for c in big:
+            c.out.fill_(3.0)
+        for c in big:     # shorter caches, other lengths per replay
+            lens = [max(x - cut, n) for x, n in zip(c.full if hasattr(c, "full") else c.lens, c.new)]
+            c.full = c.full if hasattr(c, "full") else list(c.lens)
+            c.kv.copy_(torch.tensor(lens, dtype=torch.int32))
+            c.rows = [r[:n] for r, n in zip(c.rows_full, lens)] if hasattr(c, "rows_full") else c.rows
+            if not hasattr(c, "rows_full"):
+                c.rows_full = list(c.rows)
+            c.rows = [r[:n] for r, n in zip(c.rows_full, lens)]
+            c.lens = lens
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for c in big:
+            c.check()
+    assert attn.device_status() == 0
+
+
+def test_own_workspace(dev):
+    from yllm_b200 import attn
+    c = Case(dev, 32, 8, 128, 64, [30000], [1], seed=50)
+    ws = attn.paged_workspace(128)
+    c.run(workspace=ws)
+    c.check()
+    assert bool((ws[:4096] == 0).all())      # the call leaves the counters zero
+    with pytest.raises(attn._lib.YattnError, match="workspace"):
+        c.run(workspace=ws[:4096])
+    with pytest.raises(ValueError, match="workspace"):
+        c.run(workspace=ws.cpu())
+
+
+def test_wrapper_checks(dev):
+    from yllm_b200 import attn
+    c = Case(dev, 8, 2, 64, 16, [20, 30], [1, 1], seed=51)
+    k, v = c.kp.view(-1, 16, 128), c.vp.view(-1, 16, 128)
+    good = dict(out=c.out[:, :512], q=c.q, kpool=k, vpool=v, tables=c.tables, cu_new=c.cu, kv_len=c.kv, max_new=1,
+                n_heads=8, n_kv_heads=2, head_dim=64)
+    for change, word in [
+        (dict(q=c.q.double()), "float32"), (dict(q=c.q.cpu()), "CUDA"), (dict(out=c.out[:1, :512]), "out"),
+        (dict(out=c.out[:, :512].half()), "out"), (dict(kpool=k.float()), "pool"), (dict(vpool=v[:1]), "pool"),
+        (dict(kpool=k[:, ::2]), "pool"), (dict(n_kv_heads=4, n_heads=8), "shorter"), (dict(tables=c.tables[:1]), "tables"),
+        (dict(tables=c.tables.long()), "tables"), (dict(tables=c.tables.t()), "tables"), (dict(cu_new=c.cu[:2]), "cu_new"),
+        (dict(cu_new=c.cu.long()), "cu_new"), (dict(gate=c.q[:1]), "gate"), (dict(kv_len=c.kv.cpu()), "kv_len"),
+    ]:
+        with pytest.raises(ValueError, match=word):
+            attn.attn_paged(**dict(good, **change))
+    attn.attn_paged(**dict(good, q=c.q[:0], out=c.out[:0, :512]))      # no tokens: nothing to do
+
+
+def test_pool_past_32_bits(dev):
+    """Pages whose elements lie beyond 2^32 of the pool's base."""
+    from yllm_b200 import attn
+    H, KV, hd, page = 16, 8, 128, 64
+    n_pages = (2 ** 32 // (KV * hd) + 4096) // page        # 4.3 G elements a pool
+    kp, vp = (torch.empty(n_pages, page, KV * hd, dtype=torch.float16, device=dev) for _ in range(2))
+    L = 300
+    pages = torch.tensor([n_pages - 1, 3, n_pages - 2, 0, n_pages - 3], dtype=torch.int32, device=dev)
+    kp[pages.long()] = torch.randn(5, page, KV * hd, device=dev).half()
+    vp[pages.long()] = torch.randn(5, page, KV * hd, device=dev).half()
+    T = 40
+    q, k, v = (torch.randn(T, m * hd, device=dev) for m in (H, KV, KV))
+    pos = torch.arange(L - T, L, dtype=torch.int32, device=dev)
+    slots = (pages[(pos // page).long()] * page + pos % page).to(torch.int32)
+    qo, out, one = torch.empty_like(q), torch.empty_like(q), torch.empty_like(q[:1])
+    attn.rope_store_kv_paged(qo, q, k, v, kp, vp, slots, pos, H, KV, hd, 1, 1e6)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+    attn.attn_paged(out, qo, kp, vp, pages[None], i32([0, T]), i32([L]), T, H, KV, hd)
+    attn.attn_paged(one, qo[-1:].contiguous(), kp, vp, pages[None], i32([0, 1]), i32([L]), 1, H, KV, hd)
+    torch.cuda.synchronize()
+    kk, vv = kp[pages.long()].view(-1, KV, hd)[:L].double(), vp[pages.long()].view(-1, KV, hd)[:L].double()
+    assert bool((vv[L - T:].float() - v.view(T, KV, hd)).abs().max() <= 2.0 ** -11 * v.abs().max())
+    qq = qo.double().view(T, KV, H // KV, hd)
+    s = torch.einsum("tkgd,lkd->tkgl", qq, kk) / hd ** 0.5
+    s = s.masked_fill(torch.arange(L, device=dev)[None, None, None] > pos.long()[:, None, None, None], -np.inf)
+    want = torch.einsum("tkgl,lkd->tkgd", torch.softmax(s, -1), vv).reshape(T, H * hd)
+    assert float((out.double() - want).abs().max()) < 2e-5 and float((one.double() - want[-1:]).abs().max()) < 2e-5

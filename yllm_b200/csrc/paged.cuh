@@ -340,7 +340,7 @@ template <int BN, int ROWS> struct PagedSched {
             const long long at = before(p, q, j), us = g * W + base + at, w = before(p, q, j + 1) - at;
             if (us >= x1) return false;
             u.keys = keys(p, q, j);
-            const uint32_t nb = static_cast<uint32_t>(u.keys + BN - 1) / BN;
+            const uint32_t nb = (static_cast<uint32_t>(u.keys) + BN - 1) / BN;
             u.g = g;
             u.r = r;
             u.j = j++;
