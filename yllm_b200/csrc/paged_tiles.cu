@@ -8,8 +8,10 @@
 // activations: one plane of each (fp16 holds their q exactly; P's half step 2^-11 is below the output's own
 // rounding at bf16 and equal to it at fp16).  Each q row is scaled by a power of two into (-2, 2) first,
 // and P carries a factor 2^7 (it cancels in O / l): see row_scale() and kPUp.  The tensor core truncates where
-// it adds to an accumulator, always towards zero, so PREC sums at most 1024 keys in one and adds those sums
-// in fp32 (fold() below): over 8700 keys the error was 1.1e-5 of the result without it.
+// it adds to an accumulator, always towards zero, so PREC issues Q_lo K before Q_hi K, sums at most 256 keys
+// of P V in one accumulator and adds those sums in fp32 (the fold below).  Over 8700 keys the result was off
+// by 1.1e-5 without that, 2.6e-6 with sums of 1024 keys, 0.9e-6 with 256 (elementary fp32 operations: 1.3e-6),
+// for 1 % of the time at head_dim 128 and 15 % at 256, where the fold goes through global memory.
 //
 // One persistent CTA per SM walks its share of the schedule (paged.cuh).  Warps:
 //   0-7  softmax: row r of the tile (TMEM lane r) belongs to warps r/32 and r/32 + 4, which halve each
@@ -63,7 +65,7 @@ template <int HD, bool PREC> struct TCfg {
     // PREC: the fp32 sum of the folded O.  Beside O, or at head_dim 256, where TMEM is full, in global memory
     static constexpr bool FOLD_TMEM = HD <= 128;
     static constexpr uint32_t COL_F = COL_O + HD;
-    static constexpr uint32_t FOLD = 1024 / BN;             // blocks per fold
+    static constexpr uint32_t FOLD = 256 / BN;             // blocks per fold
     static_assert(COL_O + HD * (PREC && FOLD_TMEM ? 2 : 1) <= TMEM_COLS && NSB * BN <= static_cast<int>(COL_O), "TMEM columns");
     static_assert(!PREC || LO_SMEM || COL_QLO + HD / 2 <= COL_O, "Q_lo columns");
     static_assert(SMEM <= 232448 && sizeof(PagedUnit) <= 64, "shared memory");
@@ -293,22 +295,22 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 const uint64_t dk = dk0 + warp_uniform((ks * C::KV_BYTES) >> 4);
                 const uint32_t d = tmem + C::COL_S + warp_uniform(s_sb * BN);
                 if (elect_one()) {
-#pragma unroll
-                    for (int kk = 0; kk < HD / 16; ++kk) {
-                        const uint64_t a = dq0 + (((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4);
-                        const uint64_t b = dk + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4);
-                        umma_f16(d, a, b, IDESC_QK, kk > 0 ? 1u : 0u);
-                    }
-                    if constexpr (PREC) {   // + Q_lo K^T
+                    if constexpr (PREC) {   // Q_lo K^T first: the accumulator's truncations are relative to what it holds
 #pragma unroll
                         for (int kk = 0; kk < HD / 16; ++kk) {
                             const uint64_t b = dk + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4);
                             if constexpr (C::LO_SMEM)
                                 umma_f16(d, dq0 + ((C::OFF_QLO - C::OFF_Q + (kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4), b,
-                                         IDESC_QK, 1u);
+                                         IDESC_QK, kk > 0 ? 1u : 0u);
                             else
-                                umma_f16_ts(d, tmem + C::COL_QLO + 8 * kk, b, IDESC_QK, 1u);
+                                umma_f16_ts(d, tmem + C::COL_QLO + 8 * kk, b, IDESC_QK, kk > 0 ? 1u : 0u);
                         }
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk) {
+                        const uint64_t a = dq0 + (((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4);
+                        const uint64_t b = dk + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4);
+                        umma_f16(d, a, b, IDESC_QK, PREC || kk > 0 ? 1u : 0u);
                     }
                     umma_commit(&bars->s_full[s_sb]);
                     umma_commit(&bars->k_empty[ks]);
