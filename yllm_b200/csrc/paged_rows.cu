@@ -24,9 +24,10 @@
 namespace yattn {
 namespace {
 
-// p is carried as 2^15 p (l and o with it; the factor cancels in o / l): p <= 1, and the lo plane of an unscaled
-// p under 2^-3 would fall into fp16's subnormals, 2^-25 off whatever p is, which a long context adds up.
-constexpr float kPUp = 15.f;
+// p is carried as 2^7 p (l and o with it; the factor cancels in o / l): p <= 2^8, as m may be stale by 8 binades,
+// and the lo plane of an unscaled p under 2^-3 would fall into fp16's subnormals, 2^-25 off whatever p is, which a
+// long context adds up.
+constexpr float kPUp = 7.f;
 
 template <int HD> struct RowsCfg {
     static constexpr int NCW = HD >= 256 ? 4 : 8;                // consumer warps
@@ -34,9 +35,7 @@ template <int HD> struct RowsCfg {
     static constexpr int STAGE = 2 * 16 * NCW * HD * 2;          // K and V of 16 tokens per consumer warp
     static constexpr int NST = HD <= 64 ? 5 : 3;
     static constexpr int HC_MAX = HD <= 128 ? 2 : 1;             // kv heads per unit
-    static constexpr int PT_BYTES = 2 * 8 * 48;                  // per warp: P^T hi and lo, 8 rows x 16 tokens
-    static constexpr int OFF_PT = NST * STAGE;
-    static constexpr int OFF_ML = OFF_PT + NCW * PT_BYTES;       // [NCW][8][2] floats
+    static constexpr int OFF_ML = NST * STAGE;                   // [NCW][8][2] floats
     static constexpr int NU = 4;                                 // unit descriptors in flight
     static constexpr int OFF_UNIT = OFF_ML + NCW * 8 * 2 * 4;    // [NU] units, 64 B apart
     static constexpr int OFF_BAR = OFF_UNIT + NU * 64;
@@ -158,9 +157,6 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
     // ================= consumers =================
     const uint32_t hl = warp % HC, sl = warp / HC;            // kv head of the unit, 16-token slice of a stage
     const int g8 = lane >> 2, t4 = lane & 3;                  // fragment row (token, dim, query row), column pair
-    uint8_t* pt = smem + C::OFF_PT + warp * C::PT_BYTES;
-    const uint32_t pt_u = smem_u32(pt);
-    const uint32_t p_off = (lane & 7) * 48 + ((lane >> 3) & 1) * 16;
     const uint32_t rk = 16 * sl + (lane & 15), rv = 16 * sl + (lane & 7) + ((lane >> 4) & 1) * 8;
     const uint32_t hpan = hl * (HD / 64);
     // a tile is 1024-byte atoms (8 rows of a 64-dim panel, 16-byte chunk c of row r at c ^ (r & 7)), panels then
@@ -260,46 +256,48 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                 const int32_t k0 = key0 + g8, k1 = k0 + 8;
                 const float s0 = k0 < see_a ? sc[0] * sc_a : -INFINITY, s1 = k0 < see_b ? sc[1] * sc_b : -INFINITY;
                 const float s2 = k1 < see_a ? sc[2] * sc_a : -INFINITY, s3 = k1 < see_b ? sc[3] * sc_b : -INFINITY;
-                float mx_a = fmaxf(s0, s2), mx_b = fmaxf(s1, s3);
+                // m moves only where a score passes it by more than 8 binades: rarely, and then with all that hangs on it
+                const bool grow = fmaxf(s0, s2) > m_a + 8.f || fmaxf(s1, s3) > m_b + 8.f;
+                if (__any_sync(0xffffffffu, grow)) {
+                    float mx_a = fmaxf(m_a, fmaxf(s0, s2)), mx_b = fmaxf(m_b, fmaxf(s1, s3));
 #pragma unroll
-                for (int o = 4; o <= 16; o <<= 1) {
-                    mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, o));
-                    mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, o));
+                    for (int o = 4; o <= 16; o <<= 1) {
+                        mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, o));
+                        mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, o));
+                    }
+                    // (a row that has seen no key yet keeps m = -inf)
+                    const float al_a = mx_a == -INFINITY ? 1.f : ex2_approx(m_a - mx_a);
+                    const float al_b = mx_b == -INFINITY ? 1.f : ex2_approx(m_b - mx_b);
+                    m_a = mx_a;
+                    m_b = mx_b;
+                    l_a *= al_a;
+                    l_b *= al_b;
+#pragma unroll
+                    for (int mt = 0; mt < KS; ++mt) {
+                        oc[mt][0] *= al_a;
+                        oc[mt][1] *= al_b;
+                        oc[mt][2] *= al_a;
+                        oc[mt][3] *= al_b;
+                    }
                 }
-                const float mn_a = fmaxf(m_a, mx_a), mn_b = fmaxf(m_b, mx_b);
-                // a row that has seen no key yet keeps m = -inf, and p = 0 for all its keys
-                const float ms_a = mn_a == -INFINITY ? 0.f : mn_a, ms_b = mn_b == -INFINITY ? 0.f : mn_b;
-                const float al_a = ex2_approx(m_a - ms_a), al_b = ex2_approx(m_b - ms_b);
-                const float mp_a = ms_a - kPUp, mp_b = ms_b - kPUp;
+                const float mp_a = (m_a == -INFINITY ? 0.f : m_a) - kPUp, mp_b = (m_b == -INFINITY ? 0.f : m_b) - kPUp;
                 const float p0 = ex2_approx(s0 - mp_a), p1 = ex2_approx(s1 - mp_b);
                 const float p2 = ex2_approx(s2 - mp_a), p3 = ex2_approx(s3 - mp_b);
                 // row sums stay per lane (this lane's tokens); the lanes of a column add up at the unit's end
-                l_a = l_a * al_a + (p0 + p2);
-                l_b = l_b * al_b + (p1 + p3);
-                m_a = mn_a;
-                m_b = mn_b;
-                // ---- P^T (rows x 16 tokens, 48 B row stride) as fp16 hi and lo planes ----
+                l_a += p0 + p2;
+                l_b += p1 + p3;
+                // P^T as the MMA's B operand, fp16 hi and lo planes: tokens x rows to rows x tokens, 8 x 8 at a time
+                uint32_t ph0, ph1, pl0, pl1;
                 {
                     uint32_t h01, l01, h23, l23;
                     split_h2(p0, p1, h01, l01);
                     split_h2(p2, p3, h23, l23);
-                    uint16_t* hp = reinterpret_cast<uint16_t*>(pt);
-                    uint16_t* lp = reinterpret_cast<uint16_t*>(pt + 384);
-                    const int ra = (2 * t4) * 24, rb = (2 * t4 + 1) * 24;
-                    hp[ra + g8] = static_cast<uint16_t>(h01);
-                    hp[rb + g8] = static_cast<uint16_t>(h01 >> 16);
-                    hp[ra + g8 + 8] = static_cast<uint16_t>(h23);
-                    hp[rb + g8 + 8] = static_cast<uint16_t>(h23 >> 16);
-                    lp[ra + g8] = static_cast<uint16_t>(l01);
-                    lp[rb + g8] = static_cast<uint16_t>(l01 >> 16);
-                    lp[ra + g8 + 8] = static_cast<uint16_t>(l23);
-                    lp[rb + g8 + 8] = static_cast<uint16_t>(l23 >> 16);
+                    ph0 = movmatrix_t(h01);
+                    ph1 = movmatrix_t(h23);
+                    pl0 = movmatrix_t(l01);
+                    pl1 = movmatrix_t(l23);
                 }
-                __syncwarp();
-                uint32_t ph0, ph1, pl0, pl1;
-                ldsm_x2(pt_u + p_off, ph0, ph1);
-                ldsm_x2(pt_u + 384 + p_off, pl0, pl1);
-                // ---- O^T = O^T * alpha + V^T P^T.  V rows behind the request's last key hold whatever the page
+                // ---- O^T = O^T + V^T P^T.  V rows behind the request's last key hold whatever the page
                 // held (or nothing was copied): 0 * NaN would poison the sum, so those lanes are zeroed. ----
                 uint32_t vm01 = 0xffffffffu, vm23 = 0xffffffffu;
                 if (nvalid < 16) {
@@ -319,12 +317,9 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                     float d[4] = {};
                     mma16816(d, a, pl0, pl1);
                     mma16816(d, a, ph0, ph1);
-                    oc[mt][0] = fmaf(oc[mt][0], al_a, d[0]);
-                    oc[mt][1] = fmaf(oc[mt][1], al_b, d[1]);
-                    oc[mt][2] = fmaf(oc[mt][2], al_a, d[2]);
-                    oc[mt][3] = fmaf(oc[mt][3], al_b, d[3]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) oc[mt][r] += d[r];
                 }
-                __syncwarp();   // P^T is rewritten by the next step
             }
             __syncwarp();
             if (lane == 0 && i + 1 < nt) mbar_arrive(&empty[s]);   // the last stage: after the merge below
