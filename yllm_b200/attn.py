@@ -410,6 +410,8 @@ _F16_BITS = (torch.float16, torch.uint16, torch.int16)
 
 _tls = threading.local()   # err: this thread's message buffer
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_cur_dev = torch._C._cuda_getDevice                       # (torch.cuda's wrappers of these cost as much as a launch)
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
 def _call_on(name: str, dev: int, stream, *args) -> None:
@@ -425,7 +427,7 @@ def _call_on(name: str, dev: int, stream, *args) -> None:
         err = _tls.err
     except AttributeError:
         err = _tls.err = C.create_string_buffer(512)
-    if dev == torch.cuda.current_device():
+    if dev == _cur_dev():
         rc = getattr(lib, name)(*args, raw, err, 512)
     else:
         with torch.cuda.device(dev):
@@ -546,10 +548,10 @@ def _paged_workspace(head_dim: int, dev: int, stream) -> torch.Tensor:
     if stream is not None:
         with torch.cuda.stream(stream):
             return _paged_workspace(head_dim, dev, None)
-    if torch.cuda.current_device() != dev:
+    if _cur_dev() != dev:
         with torch.cuda.device(dev):
             return _paged_workspace(head_dim, dev, None)
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         return paged_workspace(head_dim, torch.device("cuda", dev))
     key = (dev, _raw_stream(dev), head_dim)
     ws = _paged_ws.get(key)
