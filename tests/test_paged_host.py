@@ -78,7 +78,7 @@ ATTN = dict(out=P, out_stride=512, q=P, q_stride=512, gate=None, gate_stride=0, 
     (dict(ws=P + 8), "aligned"), (dict(cu_new=P + 1), "aligned"), (dict(max_pages=0), "table"),
     (dict(table_stride=3), "table"), (dict(max_pages=1 << 27, table_stride=1 << 27), "table"), (dict(n_pages=0), "2^31"),
     (dict(n_pages=1 << 27), "2^31"), (dict(n_seqs=65536), "requests"), (dict(n_tokens=1 << 30), "tokens"),
-    (dict(ws=None), "workspace"), (dict(ws_bytes=4096), "workspace"),
+    (dict(n_tokens=1 << 28, max_pages=1 << 26, table_stride=1 << 26), "divide"), (dict(ws=None), "workspace"), (dict(ws_bytes=4096), "workspace"),
 ])
 def test_attn_refuses(change, word):
     _refused("yattn_attn_paged", list(dict(ATTN, **change).values()), word)

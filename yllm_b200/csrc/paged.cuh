@@ -230,16 +230,23 @@ template <int BN, int ROWS> struct PagedSched {
     __device__ __forceinline__ uint32_t cut(long long x, long long us, long long w, uint32_t nb) const {
         const long long y = x - us - unit_cost(p);
         if (x >= us + w || y >= static_cast<long long>(nb) * block_cost(p)) return nb;
-        const uint32_t t = y <= 0 ? 0u : static_cast<uint32_t>(ROWS ? div_pos(y, block_cost(p)) : y / BN);
+        if (y <= 0) return 0;
+        const long long b = y / BN;                      // (BN is a power of two)
+        const uint32_t t = !ROWS ? static_cast<uint32_t>(b)
+                           : (b >> 31) == 0 ? div_group(p, static_cast<uint32_t>(b)) : static_cast<uint32_t>(b / p.group);
         return t < kSnap ? 0u : nb - t < kSnap ? nb : t;
     }
-    // The first CTA whose share ends at x or behind it.
+    // The first CTA whose share ends at x or behind it (0 < x <= total).
     __device__ __forceinline__ uint32_t ends_at(long long x) const {
-        uint32_t c = 0;
-#pragma unroll 1
-        for (uint32_t k = 0; k < n_active; k += 32)
-            c += __popc(__ballot_sync(0xffffffffu, k + lane < n_active && border(k + lane + 1) < x));
-        return c;
+        const long long head = (per + 1) * rem;       // where the longer shares end
+        const long long c = x <= head ? div_pos(x + per, per + 1) : rem + div_pos(x - head + per - 1, per);
+        return static_cast<uint32_t>(c) - 1;
+    }
+    // A sum over the warp of values below 2^51 (the call checks that), in two parts, one reduction instruction each.
+    static __device__ __forceinline__ long long warp_sum(long long x) {
+        const uint32_t lo = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(x) & 0xffffffu);
+        const uint32_t hi = __reduce_add_sync(0xffffffffu, static_cast<uint32_t>(x >> 24));
+        return (static_cast<long long>(hi) << 24) + lo;
     }
 
     // This CTA's share and the unit it starts in; false: no share.
@@ -256,11 +263,8 @@ template <int BN, int ROWS> struct PagedSched {
             sum += w;
             units += tiles(p, q);
         }
-#pragma unroll 1                                  // (rolled: this runs once, and its instructions are fetched cold)
-        for (int o = 16; o > 0; o >>= 1) {
-            sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            units += __shfl_xor_sync(0xffffffffu, units, o);
-        }
+        sum = warp_sum(sum);
+        units = __reduce_add_sync(0xffffffffu, units);
         W = sum;
         if (W == 0) return false;
         total = W * p.n_groups;
@@ -279,7 +283,7 @@ template <int BN, int ROWS> struct PagedSched {
         bool found = false;
         auto look = [&](uint32_t chunk, long long w) {
             long long s = w;
-#pragma unroll 1
+#pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const long long u = __shfl_up_sync(0xffffffffu, s, o);
                 if (lane >= o) s += u;
@@ -297,14 +301,17 @@ template <int BN, int ROWS> struct PagedSched {
 #pragma unroll 1
         for (uint32_t chunk = 0; !found && chunk < p.n_seqs; chunk += 32)
             look(chunk, chunk == 0 ? first : chunk + lane < p.n_seqs ? weight(p, paged_req(p, chunk + lane)) : 0);
-        // the tile of r that holds y: before() grows with t
+        // the tile of r that holds y: before() is quadratic in t, so its root (rounded) and a step or two
         j = 0;
         if (ROWS) {
             const PagedReq q = paged_req(p, r);
-            uint32_t hi = tiles(p, q);
-            while (hi - j > 1) {
-                const uint32_t mid = (j + hi) / 2;
-                if (base + before(p, q, mid) <= y) j = mid; else hi = mid;
+            const uint32_t nt = tiles(p, q);
+            if (nt > 1) {
+                const long long in = y - base;
+                const float a = static_cast<float>(before(p, q, 1)) * (1.0f / ROWS), c = static_cast<float>(in) * (2.0f / ROWS);
+                j = min(nt - 1, static_cast<uint32_t>(c / (a + sqrtf(a * a + c))));
+                while (j + 1 < nt && before(p, q, j + 1) <= in) ++j;
+                while (before(p, q, j) > in) --j;
             }
         }
         return true;

@@ -73,6 +73,13 @@ int attn_paged(void* out, uint32_t out_stride, const void* q, uint32_t q_stride,
         set_err(err, errlen, "attn_paged: too many requests (%u, at most 65535) or tokens (%u)", n_seqs, n_tokens);
         return -1;
     }
+    // the schedule's weights (paged.cuh) are summed in 51 bits
+    const double tiles = static_cast<double>(n_tokens) * (n_heads / n_kv) / kPagedTileRows + n_seqs;
+    if (tiles * (static_cast<double>(max_pages) * page_size + 1024.0) * n_heads > 1e15) {
+        set_err(err, errlen, "attn_paged: %u tokens over tables of %u pages: more work than one call can divide", n_tokens,
+                max_pages);
+        return -1;
+    }
     if (!ws || ws_bytes < workspace_bytes(hd)) {
         set_err(err, errlen, "attn_paged: workspace of %zu bytes, %zu needed", ws ? ws_bytes : static_cast<size_t>(0),
                 workspace_bytes(hd));

@@ -84,6 +84,9 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
         *abort_flag = 0;
         fence_mbar_init();
     }
+    // (the producer looks for its share meanwhile)
+    Sched sched(p);
+    const bool share = warp == NCW && sched.begin();
     __syncthreads();
 
     if (warp == NCW) {
@@ -100,7 +103,6 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
         const bool mine = i_pg < per_block;
         uint32_t gi = 0, ui = 0;
         bool ok = true;
-        Sched sched(p);
         auto publish = [&](const PagedUnit& u) -> bool {
             if (ui >= static_cast<uint32_t>(NU) &&
                 !warp_wait_bounded(&u_empty[ui % NU], ((ui / NU) & 1u) ^ 1u, p.status, ST_PAGED_TIMEOUT, abort_flag))
@@ -117,7 +119,6 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
             return gi < static_cast<uint32_t>(NST) ||
                    warp_wait_bounded(&empty[s], ((gi / NST) & 1u) ^ 1u, p.status, ST_PAGED_TIMEOUT, abort_flag);
         };
-        const bool share = sched.begin();
         while (ok && share && sched.next(u)) {
             ok = publish(u);
             if (!ok) break;

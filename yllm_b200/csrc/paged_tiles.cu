@@ -164,6 +164,8 @@ __global__ void __launch_bounds__(kTThreads, 1)
         fence_mbar_init();
     }
     if (warp == 0) tmem_alloc(&bars->tmem_base, C::TMEM_COLS);
+    Sched sched(p);                              // (its warp looks for the share meanwhile)
+    bool more = warp == 11 && sched.begin();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -185,8 +187,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
     if (warp == 11) {
         // ================= schedule =================
         uint32_t ui = 0;
-        Sched sched(p);
-        bool ok = true, more = sched.begin();
+        bool ok = true;
         for (;;) {
             PagedUnit u;
             more = more && sched.next(u);
