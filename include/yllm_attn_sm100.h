@@ -542,8 +542,9 @@ int yattn_page_step(int32_t* kv_len_out, int32_t* cu_new, int32_t* slots, int32_
  * the engine's f32_to_f16.  q, k, v and q_out hold activations of type `act`
  * (YATTN_ACT_*), heads contiguous, tokens *_stride elements apart (so q, k and
  * v may be columns of one projection output); q_out may be q itself with the
- * same stride.  A token with slot < 0 is skipped: nothing of it is written.  A slot outside the pool's n_rows rows is not stored and sets
- * device status 602.  Two tokens with one slot: either may remain.
+ * same stride.  A token with slot < 0 is skipped: nothing of it is written.  A
+ * slot outside the pool's n_rows rows is not stored and sets device status 602.
+ * Two tokens with one slot leave a mix of their rows.
  * rope_kind, n_rope_dims (kind 2: a multiple of 16) and qk_norm as
  * yattn_rope_store_kv, but the angle position*theta^(-2j/n) is taken in 64
  * bits (that call's fp32 angle drifts by half an ulp of itself at far
@@ -571,7 +572,8 @@ int yattn_rope_store_kv_paged(void* q_out, uint32_t q_out_stride, const void* q,
  * more run 128-row tiles on tcgen05.  Work is divided evenly over the SMs from
  * the lengths on the device, so nothing here depends on them at capture time.
  * fp32 activations keep about 22 bits of q and of the softmax weights (fp16 hi
- * + lo planes); 16-bit activations run one plane of each in the tiles form.
+ * + lo planes); 16-bit activations run one plane of each in the tiles form
+ * (bf16 q to 2^-19 or better of its row's largest).
  * A block table entry outside the pool reads as zero rows (device status 602);
  * a request whose offsets or lengths contradict the arguments, or which has
  * more than max_new tokens, is skipped, its rows of out not written (603).

@@ -251,6 +251,20 @@ def test_tiles_far_q(dev, act, scale):
 
 # ------------------------------------------------------- what the calls refuse or report
 
+def test_tiles_small_bf16_q_large_keys(dev):
+    """bf16 q under fp16's normal range, halfway between two of its subnormals, against keys near fp16's largest: a
+    plain conversion of q would be off by 2^-5 of it, scores of 0.67 by 0.02 and the outputs by 0.01."""
+    c = Case(dev, 8, 2, 128, 16, [200, 130], [100, 130], "bf16", seed=19)
+    c.q.fill_(2.0 ** -20 + 2.0 ** -25)
+    c.q[::3] *= -1
+    for rows in c.rows:
+        sign = torch.where(torch.arange(len(rows), device=dev) % 2 == 0, 1.0, -1.0).half()[:, None]
+        c.kp[rows] = (60000 * sign).expand(-1, c.kp.shape[1])
+        c.vp[rows] = sign.expand(-1, c.vp.shape[1]).contiguous()
+    c.run()
+    c.check()
+
+
 def test_bad_page_reads_as_zeros_and_is_reported(dev):
     """A block table entry outside the pool: status 602, and the other requests are untouched by it."""
     from yllm_b200 import attn

@@ -183,207 +183,207 @@ __global__ void __launch_bounds__(kTThreads, 1)
     };
     // registers move to the softmax warps (the launcher checks the sum against the launch's)
     if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
-    if (warp == 11) {
-        // ================= schedule =================
-        uint32_t ui = 0;
-        bool ok = true;
-        for (;;) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
+        if (warp == 11) {
+            // ================= schedule =================
+            uint32_t ui = 0;
+            bool ok = true;
+            for (;;) {
+                PagedUnit u;
+                more = more && sched.next(u);
+                if (ui >= NU)
+                    ok = warp_wait_bounded(&bars->u_empty[ui % NU], ((ui / NU) & 1u) ^ 1u, status, ST_PAGED_TIMEOUT, abort_flag);
+                if (ok && lane == 0) {
+                    u.done = more ? 0u : 1u;
+                    *unit_at(ui) = u;
+                    mbar_arrive(&bars->u_full[ui % NU]);
+                }
+                if (!ok || !more) break;
+                // its rows of q and of the gate on their way to L2, a few units ahead of their use
+                const uint32_t row0 = u.j * BM, rows = min(static_cast<uint32_t>(BM), static_cast<uint32_t>(u.n) * p.group - row0);
+#pragma unroll 1
+                for (uint32_t i = lane; i < rows; i += 32) {
+                    const uint32_t tk = div_group(p, row0 + i);
+                    const size_t tok = static_cast<size_t>(u.tok0) + tk, col = (u.g * p.group + row0 + i - tk * p.group) * HD;
+                    constexpr int ES = PREC ? 4 : 2;
+                    const char* q = static_cast<const char*>(p.q) + (tok * p.q_stride + col) * ES;
+                    const char* gt = static_cast<const char*>(p.gate) + (tok * p.gate_stride + col) * ES;
+#pragma unroll 1
+                    for (int c = 0; c < HD * ES; c += 128) {
+                        prefetch_l2(q + c);
+                        if (p.gate) prefetch_l2(gt + c);
+                    }
+                }
+                ++ui;
+            }
+        } else if (warp == 8 || warp == 10) {
+            // ================= K / V copies =================
+            const bool is_v = warp == 10;
+            const CUtensorMap* map = is_v ? &tmV : &tmK;
+            uint8_t* ring = is_v ? sV : sK;
+            uint64_t* full = is_v ? bars->v_full : bars->k_full;
+            uint64_t* empty = is_v ? bars->v_empty : bars->k_empty;
+            const uint32_t depth = is_v ? VST : KST;
+            if (lane == 0) prefetch_tensormap(map);
+            const uint32_t page = 1u << p.page_shift, box = min(page, static_cast<uint32_t>(BN));
+            const uint32_t i_pg = lane;                               // this lane's page of a block (8 at most)
+            const bool mine = i_pg < BN / box;
+            uint32_t s = 0, ph = 0, issued = 0;                       // ring stage, its pass's parity, blocks in all
+            bool ok = true;
             PagedUnit u;
-            more = more && sched.next(u);
-            if (ui >= NU)
-                ok = warp_wait_bounded(&bars->u_empty[ui % NU], ((ui / NU) & 1u) ^ 1u, status, ST_PAGED_TIMEOUT, abort_flag);
-            if (ok && lane == 0) {
-                u.done = more ? 0u : 1u;
-                *unit_at(ui) = u;
-                mbar_arrive(&bars->u_full[ui % NU]);
-            }
-            if (!ok || !more) break;
-            // its rows of q and of the gate on their way to L2, a few units ahead of their use
-            const uint32_t row0 = u.j * BM, rows = min(static_cast<uint32_t>(BM), static_cast<uint32_t>(u.n) * p.group - row0);
-#pragma unroll 1
-            for (uint32_t i = lane; i < rows; i += 32) {
-                const uint32_t tk = div_group(p, row0 + i);
-                const size_t tok = static_cast<size_t>(u.tok0) + tk, col = (u.g * p.group + row0 + i - tk * p.group) * HD;
-                constexpr int ES = PREC ? 4 : 2;
-                const char* q = static_cast<const char*>(p.q) + (tok * p.q_stride + col) * ES;
-                const char* gt = static_cast<const char*>(p.gate) + (tok * p.gate_stride + col) * ES;
-#pragma unroll 1
-                for (int c = 0; c < HD * ES; c += 128) {
-                    prefetch_l2(q + c);
-                    if (p.gate) prefetch_l2(gt + c);
+            for (uint32_t ui = 0; ok && get_unit(ui, u); ++ui) {
+                const uint32_t kend = static_cast<uint32_t>(u.keys);
+                auto row_of = [&](uint32_t b) -> int32_t {
+                    const uint32_t key = b * BN + i_pg * box;
+                    if (!mine || key >= kend) return -1;
+                    return paged_row(p, u.r, key >> p.page_shift) + static_cast<int32_t>(key & (page - 1));
+                };
+                int32_t row = u.kb1 > u.kb0 ? row_of(u.kb0) : -1;
+                for (uint32_t b = u.kb0; b < u.kb1; ++b) {
+                    if (issued >= depth &&
+                        !warp_wait_bounded(&empty[s], ph ^ 1u, status, ST_PAGED_TIMEOUT, abort_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t n_copy = __popc(__ballot_sync(0xffffffffu, row >= 0));
+                    if (lane == 0) mbar_arrive_expect_tx(&full[s], n_copy * box * (HD * 2));
+                    __syncwarp();
+                    if (row >= 0)
+                        tma_load_4d(ring + s * C::KV_BYTES + i_pg * box * (HD * 2), map, 0, 0, static_cast<int32_t>(u.g * NPAN),
+                                    row >> 3, &full[s]);
+                    ++issued;
+                    if (++s == depth) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                    row = b + 1 < u.kb1 ? row_of(b + 1) : -1;
                 }
-            }
-            ++ui;
-        }
-    } else if (warp == 8 || warp == 10) {
-        // ================= K / V copies =================
-        const bool is_v = warp == 10;
-        const CUtensorMap* map = is_v ? &tmV : &tmK;
-        uint8_t* ring = is_v ? sV : sK;
-        uint64_t* full = is_v ? bars->v_full : bars->k_full;
-        uint64_t* empty = is_v ? bars->v_empty : bars->k_empty;
-        const uint32_t depth = is_v ? VST : KST;
-        if (lane == 0) prefetch_tensormap(map);
-        const uint32_t page = 1u << p.page_shift, box = min(page, static_cast<uint32_t>(BN));
-        const uint32_t i_pg = lane;                               // this lane's page of a block (8 at most)
-        const bool mine = i_pg < BN / box;
-        uint32_t s = 0, ph = 0, issued = 0;                       // ring stage, its pass's parity, blocks in all
-        bool ok = true;
-        PagedUnit u;
-        for (uint32_t ui = 0; ok && get_unit(ui, u); ++ui) {
-            const uint32_t kend = static_cast<uint32_t>(u.keys);
-            auto row_of = [&](uint32_t b) -> int32_t {
-                const uint32_t key = b * BN + i_pg * box;
-                if (!mine || key >= kend) return -1;
-                return paged_row(p, u.r, key >> p.page_shift) + static_cast<int32_t>(key & (page - 1));
-            };
-            int32_t row = u.kb1 > u.kb0 ? row_of(u.kb0) : -1;
-            for (uint32_t b = u.kb0; b < u.kb1; ++b) {
-                if (issued >= depth &&
-                    !warp_wait_bounded(&empty[s], ph ^ 1u, status, ST_PAGED_TIMEOUT, abort_flag)) {
-                    ok = false;
-                    break;
-                }
-                const uint32_t n_copy = __popc(__ballot_sync(0xffffffffu, row >= 0));
-                if (lane == 0) mbar_arrive_expect_tx(&full[s], n_copy * box * (HD * 2));
-                __syncwarp();
-                if (row >= 0)
-                    tma_load_4d(ring + s * C::KV_BYTES + i_pg * box * (HD * 2), map, 0, 0, static_cast<int32_t>(u.g * NPAN),
-                                row >> 3, &full[s]);
-                ++issued;
-                if (++s == depth) {
-                    s = 0;
-                    ph ^= 1u;
-                }
-                row = b + 1 < u.kb1 ? row_of(b + 1) : -1;
-            }
-            put_unit(ui);
-        }
-        // no copy may still be landing when the CTA exits
-        volatile int dummy = 0;
-        for (uint32_t b = issued > depth ? issued - depth : 0; b < issued; ++b)
-            mbar_wait_bounded(&full[b % depth], (b / depth) & 1u, status, ST_PAGED_TIMEOUT, &dummy);
-    } else {
-        // ================= MMA =================
-        constexpr uint32_t IDESC_QK = idesc_f16(BM, BN, 0);
-        constexpr uint32_t IDESC_PV = idesc_f16(BM, HD, 1);
-        // an operand at base + off has the base's descriptor + off / 16
-        const uint64_t dq0 = sdesc_sw128(sQ, 16, 1024);
-        // K and V tiles: 1024-byte atoms of 8 rows x 64 dims, panels 1024 B and row groups NPAN * 1024 B apart
-        const uint64_t dk0 = sdesc_sw128(sK, 16, NPAN * 1024);
-        const uint64_t dv0 = sdesc_sw128(sV, 1024, NPAN * 1024);
-        uint32_t ks = 0, kph = 0, vs = 0, vph = 0;      // ring stages and parities
-        uint32_t s_sb = 0, pv_sb = 0, pv_ph = 0;        // S buffer of the next S product, of the next PV product
-        uint32_t qph = 0;
-        bool ok = true;
-        PagedUnit u;
-        for (uint32_t ui = 0; ok && get_unit(ui, u); ++ui) {
-            const uint32_t nb = u.kb1 - u.kb0;
-            if (nb == 0) {
                 put_unit(ui);
-                continue;
             }
-            const int32_t kend = u.keys;
-            ok = warp_wait_bounded(&bars->q_full, qph, status, ST_PAGED_TIMEOUT, abort_flag);
-            qph ^= 1u;
-            tc_fence_after();
-            // S = Q K^T of the next block into the next S buffer; that buffer's last P was consumed by a PV product
-            // issued earlier, and the tensor core runs one thread's MMAs in order
-            auto do_s = [&]() -> bool {
-                if (!warp_wait_bounded(&bars->k_full[ks], kph, status, ST_PAGED_TIMEOUT, abort_flag)) return false;
+            // no copy may still be landing when the CTA exits
+            volatile int dummy = 0;
+            for (uint32_t b = issued > depth ? issued - depth : 0; b < issued; ++b)
+                mbar_wait_bounded(&full[b % depth], (b / depth) & 1u, status, ST_PAGED_TIMEOUT, &dummy);
+        } else {
+            // ================= MMA =================
+            constexpr uint32_t IDESC_QK = idesc_f16(BM, BN, 0);
+            constexpr uint32_t IDESC_PV = idesc_f16(BM, HD, 1);
+            // an operand at base + off has the base's descriptor + off / 16
+            const uint64_t dq0 = sdesc_sw128(sQ, 16, 1024);
+            // K and V tiles: 1024-byte atoms of 8 rows x 64 dims, panels 1024 B and row groups NPAN * 1024 B apart
+            const uint64_t dk0 = sdesc_sw128(sK, 16, NPAN * 1024);
+            const uint64_t dv0 = sdesc_sw128(sV, 1024, NPAN * 1024);
+            uint32_t ks = 0, kph = 0, vs = 0, vph = 0;      // ring stages and parities
+            uint32_t s_sb = 0, pv_sb = 0, pv_ph = 0;        // S buffer of the next S product, of the next PV product
+            uint32_t qph = 0;
+            bool ok = true;
+            PagedUnit u;
+            for (uint32_t ui = 0; ok && get_unit(ui, u); ++ui) {
+                const uint32_t nb = u.kb1 - u.kb0;
+                if (nb == 0) {
+                    put_unit(ui);
+                    continue;
+                }
+                const int32_t kend = u.keys;
+                ok = warp_wait_bounded(&bars->q_full, qph, status, ST_PAGED_TIMEOUT, abort_flag);
+                qph ^= 1u;
                 tc_fence_after();
-                const uint64_t dk = dk0 + warp_uniform((ks * C::KV_BYTES) >> 4);
-                const uint32_t d = tmem + C::COL_S + warp_uniform(s_sb * BN);
-                if (elect_one()) {
-                    if constexpr (PREC) {   // Q_lo K^T first: the accumulator's truncations are relative to what it holds
+                // S = Q K^T of the next block into the next S buffer; that buffer's last P was consumed by a PV product
+                // issued earlier, and the tensor core runs one thread's MMAs in order
+                auto do_s = [&]() -> bool {
+                    if (!warp_wait_bounded(&bars->k_full[ks], kph, status, ST_PAGED_TIMEOUT, abort_flag)) return false;
+                    tc_fence_after();
+                    const uint64_t dk = dk0 + warp_uniform((ks * C::KV_BYTES) >> 4);
+                    const uint32_t d = tmem + C::COL_S + warp_uniform(s_sb * BN);
+                    if (elect_one()) {
+                        if constexpr (PREC) {   // Q_lo K^T first: the accumulator's truncations are relative to what it holds
+#pragma unroll
+                            for (int kk = 0; kk < HD / 16; ++kk) {
+                                const uint64_t b = dk + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4);
+                                if constexpr (C::LO_SMEM)
+                                    umma_f16(d, dq0 + ((C::OFF_QLO - C::OFF_Q + (kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4), b,
+                                             IDESC_QK, kk > 0 ? 1u : 0u);
+                                else
+                                    umma_f16_ts(d, tmem + C::COL_QLO + 8 * kk, b, IDESC_QK, kk > 0 ? 1u : 0u);
+                            }
+                        }
 #pragma unroll
                         for (int kk = 0; kk < HD / 16; ++kk) {
+                            const uint64_t a = dq0 + (((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4);
                             const uint64_t b = dk + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4);
-                            if constexpr (C::LO_SMEM)
-                                umma_f16(d, dq0 + ((C::OFF_QLO - C::OFF_Q + (kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4), b,
-                                         IDESC_QK, kk > 0 ? 1u : 0u);
-                            else
-                                umma_f16_ts(d, tmem + C::COL_QLO + 8 * kk, b, IDESC_QK, kk > 0 ? 1u : 0u);
+                            umma_f16(d, a, b, IDESC_QK, PREC || kk > 0 ? 1u : 0u);
                         }
+                        umma_commit(&bars->s_full[s_sb]);
+                        umma_commit(&bars->k_empty[ks]);
                     }
-#pragma unroll
-                    for (int kk = 0; kk < HD / 16; ++kk) {
-                        const uint64_t a = dq0 + (((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4);
-                        const uint64_t b = dk + (((kk >> 2) * 1024 + (kk & 3) * 32) >> 4);
-                        umma_f16(d, a, b, IDESC_QK, PREC || kk > 0 ? 1u : 0u);
-                    }
-                    umma_commit(&bars->s_full[s_sb]);
-                    umma_commit(&bars->k_empty[ks]);
-                }
-                __syncwarp();
-                if (++s_sb == NSB) s_sb = 0;
-                if (++ks == KST) {
-                    ks = 0;
-                    kph ^= 1u;
-                }
-                return true;
-            };
-            // O += P V: keys [16 kk, +16) of a plane are the 8 columns at 32 (kk/2) + 16 plane + 8 (kk%2)
-            auto do_pv = [&](uint32_t jj) -> bool {
-                if (!warp_wait_bounded(&bars->p_full[pv_sb], pv_ph, status, ST_PAGED_TIMEOUT, abort_flag) ||
-                    !warp_wait_bounded(&bars->v_full[vs], vph, status, ST_PAGED_TIMEOUT, abort_flag))
-                    return false;
-                tc_fence_after();
-                const int valid = min(BN, kend - static_cast<int32_t>((u.kb0 + jj) * BN));   // >= 1
-                const int steps = (valid + 15) >> 4;
-                if (valid & 15) {   // the rest of the last 16-key step
-                    const int zrows = steps * 16 - valid;
-                    for (int i = lane; i < zrows * NPAN * 8; i += 32) {
-                        const int row = valid + i / (NPAN * 8), c = i % (NPAN * 8);
-                        *reinterpret_cast<uint4*>(sV + vs * C::KV_BYTES + ((row >> 3) * NPAN + (c >> 3)) * 1024 + (row & 7) * 128 + (c & 7) * 16) =
-                            make_uint4(0u, 0u, 0u, 0u);
-                    }
-                    fence_proxy_async_smem();
                     __syncwarp();
-                }
-                const uint32_t pcol = tmem + C::COL_S + warp_uniform(pv_sb * BN);
-                const uint64_t dv = dv0 + warp_uniform((vs * C::KV_BYTES) >> 4);
-                if (elect_one()) {
-                    const bool fresh = PREC ? jj % FOLD == 0 : jj == 0;   // PREC: the sum so far has been folded
+                    if (++s_sb == NSB) s_sb = 0;
+                    if (++ks == KST) {
+                        ks = 0;
+                        kph ^= 1u;
+                    }
+                    return true;
+                };
+                // O += P V: keys [16 kk, +16) of a plane are the 8 columns at 32 (kk/2) + 16 plane + 8 (kk%2)
+                auto do_pv = [&](uint32_t jj) -> bool {
+                    if (!warp_wait_bounded(&bars->p_full[pv_sb], pv_ph, status, ST_PAGED_TIMEOUT, abort_flag) ||
+                        !warp_wait_bounded(&bars->v_full[vs], vph, status, ST_PAGED_TIMEOUT, abort_flag))
+                        return false;
+                    tc_fence_after();
+                    const int valid = min(BN, kend - static_cast<int32_t>((u.kb0 + jj) * BN));   // >= 1
+                    const int steps = (valid + 15) >> 4;
+                    if (valid & 15) {   // the rest of the last 16-key step
+                        const int zrows = steps * 16 - valid;
+                        for (int i = lane; i < zrows * NPAN * 8; i += 32) {
+                            const int row = valid + i / (NPAN * 8), c = i % (NPAN * 8);
+                            *reinterpret_cast<uint4*>(sV + vs * C::KV_BYTES + ((row >> 3) * NPAN + (c >> 3)) * 1024 + (row & 7) * 128 + (c & 7) * 16) =
+                                make_uint4(0u, 0u, 0u, 0u);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                    }
+                    const uint32_t pcol = tmem + C::COL_S + warp_uniform(pv_sb * BN);
+                    const uint64_t dv = dv0 + warp_uniform((vs * C::KV_BYTES) >> 4);
+                    if (elect_one()) {
+                        const bool fresh = PREC ? jj % FOLD == 0 : jj == 0;   // PREC: the sum so far has been folded
 #pragma unroll
-                    for (int plane = 0; plane < (PREC ? 2 : 1); ++plane)
+                        for (int plane = 0; plane < (PREC ? 2 : 1); ++plane)
 #pragma unroll
-                        for (int kk = 0; kk < BN / 16; ++kk)
-                            if (kk < steps)
-                                umma_f16_ts(tmem + C::COL_O, pcol + 32 * (kk >> 1) + 16 * plane + 8 * (kk & 1),
-                                            dv + ((kk * 2 * NPAN * 1024) >> 4), IDESC_PV,
-                                            (!fresh || plane > 0 || kk > 0) ? 1u : 0u);
-                    umma_commit(&bars->v_empty[vs]);
-                    umma_commit(&bars->pv_done[pv_sb]);
+                            for (int kk = 0; kk < BN / 16; ++kk)
+                                if (kk < steps)
+                                    umma_f16_ts(tmem + C::COL_O, pcol + 32 * (kk >> 1) + 16 * plane + 8 * (kk & 1),
+                                                dv + ((kk * 2 * NPAN * 1024) >> 4), IDESC_PV,
+                                                (!fresh || plane > 0 || kk > 0) ? 1u : 0u);
+                        umma_commit(&bars->v_empty[vs]);
+                        umma_commit(&bars->pv_done[pv_sb]);
+                    }
+                    __syncwarp();
+                    if (++pv_sb == NSB) {
+                        pv_sb = 0;
+                        pv_ph ^= 1u;
+                    }
+                    if (++vs == VST) {
+                        vs = 0;
+                        vph ^= 1u;
+                    }
+                    return true;
+                };
+                for (uint32_t jj = 0; ok && jj < nb && jj < NSB; ++jj) ok = do_s();
+                for (uint32_t jj = 0; ok && jj < nb; ++jj) {
+                    ok = do_pv(jj);
+                    if (ok && jj + NSB < nb) ok = do_s();
                 }
-                __syncwarp();
-                if (++pv_sb == NSB) {
-                    pv_sb = 0;
-                    pv_ph ^= 1u;
-                }
-                if (++vs == VST) {
-                    vs = 0;
-                    vph ^= 1u;
-                }
-                return true;
-            };
-            for (uint32_t jj = 0; ok && jj < nb && jj < NSB; ++jj) ok = do_s();
-            for (uint32_t jj = 0; ok && jj < nb; ++jj) {
-                ok = do_pv(jj);
-                if (ok && jj + NSB < nb) ok = do_s();
+                if (ok && elect_one()) umma_commit(&bars->o_done);
+                put_unit(ui);
             }
-            if (ok && elect_one()) umma_commit(&bars->o_done);
-            put_unit(ui);
+            // every MMA issued so far completes before TMEM is freed
+            if (elect_one()) {
+                umma_commit(&bars->mma_drain);
+                volatile int dummy = 0;
+                mbar_wait_bounded(&bars->mma_drain, 0, status, ST_PAGED_TIMEOUT, &dummy);
+            }
+            __syncwarp();
         }
-        // every MMA issued so far completes before TMEM is freed
-        if (elect_one()) {
-            umma_commit(&bars->mma_drain);
-            volatile int dummy = 0;
-            mbar_wait_bounded(&bars->mma_drain, 0, status, ST_PAGED_TIMEOUT, &dummy);
-        }
-        __syncwarp();
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         // ================= softmax warps 0-7 =================
@@ -428,7 +428,8 @@ __global__ void __launch_bounds__(kTThreads, 1)
                     for (int sub = 0; sub < SUBS; ++sub) {
                         g[sub * 4 + i] = make_uint4(0u, 0u, 0u, 0u);
                         if (in)
-                            g[sub * 4 + i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(p.gate) + (token * p.gate_stride + col + sub * CW) * ES));
+                            g[sub * 4 + i] = __ldg(reinterpret_cast<const uint4*>(
+                                static_cast<const char*>(p.gate) + (token * p.gate_stride + col + sub * CW) * ES));
                     }
                 }
             };
@@ -537,293 +538,299 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 }
             };
             if (nb > 0) {
-            float up = 1.f;
-            // ---- Q, each row scaled by its power of two: hi to shared memory, lo (PREC) beside it or to TMEM ----
-            if constexpr (!PREC || C::LO_SMEM) {
-                // warp w fetches rows 16 w .. + 15, LPR lanes a row, 16 bytes a lane
-                constexpr int ES = PREC ? 4 : 2, EL = 16 / ES, LPR = HD / EL, RPI = 32 / LPR, NI = 16 / RPI;
-                uint4 raw[NI];
-#pragma unroll
-                for (int i = 0; i < NI; ++i) {
-                    const uint32_t row = warp * 16 + i * RPI + lane / LPR;
-                    const uint32_t fr = row0 + min(row, rows - 1), tr = div_group(p, fr);
-                    const size_t at = (static_cast<size_t>(u.tok0) + tr) * p.q_stride +
-                                      (u.g * p.group + fr - tr * p.group) * HD + (lane % LPR) * EL;
-                    raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + at * ES));
-                }
-                // fp16 goes as it is; bf16 too where fp16 can hold this warp's rows (below 2^15; what falls under fp16's
-                // subnormals is off by 2^-25, far below the output's rounding), else scaled as fp32 is
-                bool plain = ACT == YATTN_ACT_F16;
-                if constexpr (ACT == YATTN_ACT_BF16) {
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int i = 0; i < NI; ++i)
-                        top = max(top, max(max(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu), max(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu)));
-                    uint32_t low = 0;
-#pragma unroll
-                    for (int i = 0; i < NI; ++i)
-                        low = max(low, max(max(raw[i].x & 0x7fffu, raw[i].y & 0x7fffu), max(raw[i].z & 0x7fffu, raw[i].w & 0x7fffu)));
-                    plain = __all_sync(0xffffffffu, (top >> 16) < 0x4700u && low < 0x4700u);
-                    if (plain) {
-#pragma unroll
-                        for (int i = 0; i < NI; ++i) {
-                            uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-#pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                w[k] = h2_bits(__floats2half2_rn(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u)));
-                            raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
-                    }
-                }
-                if (plain) {
+                float up = 1.f;
+                // ---- Q, each row scaled by its power of two: hi to shared memory, lo (PREC) beside it or to TMEM ----
+                if constexpr (!PREC || C::LO_SMEM) {
+                    // warp w fetches rows 16 w .. + 15, LPR lanes a row, 16 bytes a lane
+                    constexpr int ES = PREC ? 4 : 2, EL = 16 / ES, LPR = HD / EL, RPI = 32 / LPR, NI = 16 / RPI;
+                    uint4 raw[NI];
 #pragma unroll
                     for (int i = 0; i < NI; ++i) {
                         const uint32_t row = warp * 16 + i * RPI + lane / LPR;
-                        if (lane % LPR == 0) s_up[row] = 1.f;
-                        *reinterpret_cast<uint4*>(sQ + sw128_offset(row, (lane % LPR) * EL, BM)) = raw[i];
+                        const uint32_t fr = row0 + min(row, rows - 1), tr = div_group(p, fr);
+                        const size_t at = (static_cast<size_t>(u.tok0) + tr) * p.q_stride +
+                                          (u.g * p.group + fr - tr * p.group) * HD + (lane % LPR) * EL;
+                        raw[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + at * ES));
                     }
-                } else {
+                    // fp16 goes as it is; bf16 too where fp16 holds this warp's rows: every 8 neighbours below 2^15 and, unless
+                    // all zero, with one of 2^-6 or more, so what falls under fp16's normal range is off by 2^-25, which is
+                    // 2^-19 of its row's largest (bf16 itself rounds at 2^-9).  Else scaled as fp32 is
+                    bool plain = ACT == YATTN_ACT_F16;
+                    if constexpr (ACT == YATTN_ACT_BF16) {
+                        bool fits = true;
 #pragma unroll
-                for (int i = 0; i < NI; ++i) {
-                    const uint32_t row = warp * 16 + i * RPI + lane / LPR;
-                    const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-                    float x[EL], mx = 0.f;
+                        for (int i = 0; i < NI; ++i) {
+                            uint32_t hi = 0, lo = 0;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        if constexpr (PREC) {
-                            x[k] = __uint_as_float(w[k]);
-                        } else {
-                            const float2 t = ACT == YATTN_ACT_F16
-                                                 ? h2f2(w[k])
-                                                 : make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
-                            x[2 * k] = t.x;
-                            x[2 * k + 1] = t.y;
+                            for (int k = 0; k < 4; ++k) {
+                                const uint32_t w = k == 0 ? raw[i].x : k == 1 ? raw[i].y : k == 2 ? raw[i].z : raw[i].w;
+                                hi = max(hi, w & 0x7fff7fffu);
+                                lo = max(lo, w & 0x7fffu);
+                            }
+                            const uint32_t top = max(hi >> 16, lo);   // the largest of 8 values, as bf16 bits
+                            fits = fits && (top == 0 || (top >= 0x3c80u && top < 0x4700u));
                         }
-                    }
+                        plain = __all_sync(0xffffffffu, fits);
+                        if (plain) {
 #pragma unroll
-                    for (int k = 0; k < EL; ++k) mx = fmaxf(mx, fabsf(x[k]));
-                    if constexpr (LPR == 32) {               // (magnitudes order as their bits)
-                        mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
-                    } else {
+                            for (int i = 0; i < NI; ++i) {
+                                uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-                        for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                    }
-                    float down, rup;
-                    row_scale(mx, down, rup);
-                    if (lane % LPR == 0) s_up[row] = rup;
-                    uint32_t hi[EL / 2], lo[EL / 2];
-#pragma unroll
-                    for (int k = 0; k < EL / 2; ++k) {
-                        const float a = x[2 * k] * down, b = x[2 * k + 1] * down;
-                        const __half2 hv = __floats2half2_rn(a, b);
-                        hi[k] = h2_bits(hv);
-                        const float2 fv = __half22float2(hv);
-                        lo[k] = h2_bits(__floats2half2_rn(a - fv.x, b - fv.y));
-                    }
-                    uint8_t* dst = sQ + sw128_offset(row, (lane % LPR) * EL, BM);
-                    if constexpr (PREC) {
-                        *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
-                        *reinterpret_cast<uint2*>(dst + (C::OFF_QLO - C::OFF_Q)) = make_uint2(lo[0], lo[1]);
-                    } else {
-                        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    }
-                }
-                }
-                fence_proxy_async_smem();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars->q_full);
-                named_bar_sync(5, 256);                                   // s_up of every row
-                up = s_up[r];
-            } else {
-                // head_dim 256, fp32: a row's half per lane, in two passes (its largest value, then the planes)
-                constexpr int CH = 64;                                    // columns in registers at a time
-                float x[CH];
-                const size_t qi = (static_cast<size_t>(u.tok0) + tk) * p.q_stride + hcol + h * (HD / 2);
-                auto load = [&](int c) {
-                    const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + qi + c);
-#pragma unroll
-                    for (int i = 0; i < CH / 4; ++i) {
-                        const float4 v = __ldg(src + i);
-                        x[4 * i] = v.x;
-                        x[4 * i + 1] = v.y;
-                        x[4 * i + 2] = v.z;
-                        x[4 * i + 3] = v.w;
-                    }
-                };
-                float mx = 0.f;
-#pragma unroll 1
-                for (int c = HD / 2 - CH; c >= 0; c -= CH) {              // ends with columns [0, CH) in x
-                    load(c);
-#pragma unroll
-                    for (int i = 0; i < CH; ++i) mx = fmaxf(mx, fabsf(x[i]));
-                }
-                xch[h * BM + r] = mx;
-                named_bar_sync(1 + qd, 64);                               // the row's two halves
-                mx = fmaxf(xch[r], xch[BM + r]);
-                named_bar_sync(1 + qd, 64);                               // read before the first block's maxima
-                float down;
-                row_scale(mx, down, up);
-#pragma unroll 1
-                for (int c = 0; c < HD / 2; c += CH) {
-                    if (c > 0) load(c);
-                    const int d0 = h * (HD / 2) + c;
-#pragma unroll
-                    for (int i = 0; i < CH; i += 32) {
-                        uint32_t hi[16], lo[16];
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            const float a = x[i + 2 * k] * down, b = x[i + 2 * k + 1] * down;
-                            const __half2 hv = __floats2half2_rn(a, b);
-                            hi[k] = h2_bits(hv);
-                            const float2 fv = __half22float2(hv);
-                            lo[k] = h2_bits(__floats2half2_rn(a - fv.x, b - fv.y));
-                        }
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            *reinterpret_cast<uint4*>(sQ + sw128_offset(r, d0 + i + 8 * k, BM)) =
-                                make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
-                        tmem_st16(trow + C::COL_QLO + (d0 + i) / 2, lo);
-                    }
-                }
-                tmem_wait_st();
-                fence_proxy_async_smem();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars->q_full);
-            }
-            const float sl2 = p.scale_log2 * up;
-            for (uint32_t j = 0; j < nb; ++j) {
-                const bool have = warp_wait_bounded(&bars->s_full[sb], sph, status, ST_PAGED_TIMEOUT, abort_flag);
-                if (!work) {                             // no live row: P's lanes stay as they are, nothing reads them
-                    if (!named_bar_and(1 + qd, 64, have)) {
-                        ok = false;
-                        break;
-                    }
-                } else {
-                    const uint32_t scol = trow + C::COL_S + sb * BN + h * HB;
-                    float sv[HB];
-                    if (have) {
-                        tc_fence_after();
-#pragma unroll
-                        for (int c = 0; c < HB / 32; ++c) {
-                            uint32_t rr[32];
-                            tmem_ld32(scol + c * 32, rr);
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) sv[c * 32 + i] = __uint_as_float(rr[i]);
-                        }
-                        tmem_wait_ld();
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < HB; ++c) sv[c] = -INFINITY;
-                    }
-                    // causal mask; also drops the stale rows behind the last key (their S may be NaN)
-                    const int32_t kbase = static_cast<int32_t>((u.kb0 + j) * BN) + h * HB;
-                    if (static_cast<int32_t>((u.kb0 + j + 1) * BN) - 1 > qpos_min) {
-#pragma unroll
-                        for (int c = 0; c < HB; ++c)
-                            if (kbase + c > qpos) sv[c] = -INFINITY;
-                    }
-                    float mx4[4] = {sv[0], sv[1], sv[2], sv[3]};
-#pragma unroll
-                    for (int c = 4; c < HB; c += 4) {
-                        mx4[0] = fmaxf(mx4[0], sv[c]);
-                        mx4[1] = fmaxf(mx4[1], sv[c + 1]);
-                        mx4[2] = fmaxf(mx4[2], sv[c + 2]);
-                        mx4[3] = fmaxf(mx4[3], sv[c + 3]);
-                    }
-                    float* xb = xch + (j & 1) * (2 * BM);
-                    xb[h * BM + r] = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-                    if (!named_bar_and(1 + qd, 64, have)) {
-                        ok = false;
-                        break;
-                    }
-                    const float mx = fmaxf(xb[r], xb[BM + r]) * sl2;
-                    const float m_new = fmaxf(m_run, mx);
-                    const bool grow = m_new > m_run + 8.0f;          // a stale m costs nothing up to 2^8
-                    const float m_use = grow ? m_new : m_run;
-                    const float alpha = grow ? ex2_approx(m_run - m_use) : 1.0f;
-                    const float m_sub = (m_use == -INFINITY ? 0.f : m_use) - kPUp;   // no key yet: p = 0
-                    const float2 sl2x2 = make_float2(sl2, sl2), negm = make_float2(-m_sub, -m_sub);
-                    const float2 neg1 = make_float2(-1.f, -1.f);
-                    float2 rs2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-                    for (int c = 0; c < HB / 32; ++c) {   // 32 keys: 16 columns of P hi, then 16 of P lo
-                        uint32_t hi[16], lo[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float2 x = __ffma2_rn(make_float2(sv[c * 32 + 2 * i], sv[c * 32 + 2 * i + 1]), sl2x2, negm);
-                            const float2 pp = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-                            rs2[i & 1] = __fadd2_rn(rs2[i & 1], pp);
-                            const __half2 hv = __floats2half2_rn(pp.x, pp.y);
-                            hi[i] = h2_bits(hv);
-                            if constexpr (PREC) {
-                                const float2 d = __ffma2_rn(__half22float2(hv), neg1, pp);
-                                lo[i] = h2_bits(__floats2half2_rn(d.x, d.y));
+                                for (int k = 0; k < 4; ++k)
+                                    w[k] = h2_bits(__floats2half2_rn(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u)));
+                                raw[i] = make_uint4(w[0], w[1], w[2], w[3]);
                             }
                         }
-                        tmem_st16(scol + c * 32, hi);
-                        if constexpr (PREC) tmem_st16(scol + c * 32 + 16, lo);
                     }
-                    l_run = l_run * alpha + ((rs2[0].x + rs2[0].y) + (rs2[1].x + rs2[1].y));
-                    m_run = m_use;
-                    // ---- O rescale (rare) or fold (PREC), this half's columns: the last block's PV must have
-                    // finished.  Both halves of the rows see the same `grow`. ----
-                    const bool fold = PREC && j >= 1 && j % FOLD == 0;
-                    if (j >= 1 && (fold || __any_sync(0xffffffffu, grow))) {
-                        const bool done = warp_wait_bounded(&bars->pv_done[pb], pph, status, ST_PAGED_TIMEOUT, abort_flag);
-                        if (!named_bar_and(1 + qd, 64, done)) {
-                            ok = false;
-                            break;
+                    if (plain) {
+#pragma unroll
+                        for (int i = 0; i < NI; ++i) {
+                            const uint32_t row = warp * 16 + i * RPI + lane / LPR;
+                            if (lane % LPR == 0) s_up[row] = 1.f;
+                            *reinterpret_cast<uint4*>(sQ + sw128_offset(row, (lane % LPR) * EL, BM)) = raw[i];
                         }
-                        tc_fence_after();
-                        const bool folded = PREC && j > FOLD;
-#pragma unroll 1
-                        for (int c = 0; c < HD / 2; c += 32) {
-                            float x[32];
-                            ld_o(c, x, fold && folded);
+                    } else {
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) x[i] *= alpha;
-                            if (fold) {
-                                st_fold(c, x);
-                                continue;
-                            }
-                            uint32_t rr[32];
+                        for (int i = 0; i < NI; ++i) {
+                            const uint32_t row = warp * 16 + i * RPI + lane / LPR;
+                            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                            float x[EL], mx = 0.f;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) rr[i] = __float_as_uint(x[i]);
-                            tmem_st32(ocol + c, rr);
-                            if constexpr (PREC) {
-                                if (folded) {
-                                    ld_fold(c, x);
-#pragma unroll
-                                    for (int i = 0; i < 32; ++i) x[i] *= alpha;
-                                    st_fold(c, x);
+                            for (int k = 0; k < 4; ++k) {
+                                if constexpr (PREC) {
+                                    x[k] = __uint_as_float(w[k]);
+                                } else {
+                                    const float2 t = ACT == YATTN_ACT_F16
+                                                         ? h2f2(w[k])
+                                                         : make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+                                    x[2 * k] = t.x;
+                                    x[2 * k + 1] = t.y;
                                 }
                             }
+#pragma unroll
+                            for (int k = 0; k < EL; ++k) mx = fmaxf(mx, fabsf(x[k]));
+                            if constexpr (LPR == 32) {               // (magnitudes order as their bits)
+                                mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
+                            } else {
+#pragma unroll
+                                for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                            }
+                            float down, rup;
+                            row_scale(mx, down, rup);
+                            if (lane % LPR == 0) s_up[row] = rup;
+                            uint32_t hi[EL / 2], lo[EL / 2];
+#pragma unroll
+                            for (int k = 0; k < EL / 2; ++k) {
+                                const float a = x[2 * k] * down, b = x[2 * k + 1] * down;
+                                const __half2 hv = __floats2half2_rn(a, b);
+                                hi[k] = h2_bits(hv);
+                                const float2 fv = __half22float2(hv);
+                                lo[k] = h2_bits(__floats2half2_rn(a - fv.x, b - fv.y));
+                            }
+                            uint8_t* dst = sQ + sw128_offset(row, (lane % LPR) * EL, BM);
+                            if constexpr (PREC) {
+                                *reinterpret_cast<uint2*>(dst) = make_uint2(hi[0], hi[1]);
+                                *reinterpret_cast<uint2*>(dst + (C::OFF_QLO - C::OFF_Q)) = make_uint2(lo[0], lo[1]);
+                            } else {
+                                *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            }
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars->q_full);
+                    named_bar_sync(5, 256);                                   // s_up of every row
+                    up = s_up[r];
+                } else {
+                    // head_dim 256, fp32: a row's half per lane, in two passes (its largest value, then the planes)
+                    constexpr int CH = 64;                                    // columns in registers at a time
+                    float x[CH];
+                    const size_t qi = (static_cast<size_t>(u.tok0) + tk) * p.q_stride + hcol + h * (HD / 2);
+                    auto load = [&](int c) {
+                        const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + qi + c);
+#pragma unroll
+                        for (int i = 0; i < CH / 4; ++i) {
+                            const float4 v = __ldg(src + i);
+                            x[4 * i] = v.x;
+                            x[4 * i + 1] = v.y;
+                            x[4 * i + 2] = v.z;
+                            x[4 * i + 3] = v.w;
+                        }
+                    };
+                    float mx = 0.f;
+#pragma unroll 1
+                    for (int c = HD / 2 - CH; c >= 0; c -= CH) {              // ends with columns [0, CH) in x
+                        load(c);
+#pragma unroll
+                        for (int i = 0; i < CH; ++i) mx = fmaxf(mx, fabsf(x[i]));
+                    }
+                    xch[h * BM + r] = mx;
+                    named_bar_sync(1 + qd, 64);                               // the row's two halves
+                    mx = fmaxf(xch[r], xch[BM + r]);
+                    named_bar_sync(1 + qd, 64);                               // read before the first block's maxima
+                    float down;
+                    row_scale(mx, down, up);
+#pragma unroll 1
+                    for (int c = 0; c < HD / 2; c += CH) {
+                        if (c > 0) load(c);
+                        const int d0 = h * (HD / 2) + c;
+#pragma unroll
+                        for (int i = 0; i < CH; i += 32) {
+                            uint32_t hi[16], lo[16];
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) {
+                                const float a = x[i + 2 * k] * down, b = x[i + 2 * k + 1] * down;
+                                const __half2 hv = __floats2half2_rn(a, b);
+                                hi[k] = h2_bits(hv);
+                                const float2 fv = __half22float2(hv);
+                                lo[k] = h2_bits(__floats2half2_rn(a - fv.x, b - fv.y));
+                            }
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                *reinterpret_cast<uint4*>(sQ + sw128_offset(r, d0 + i + 8 * k, BM)) =
+                                    make_uint4(hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
+                            tmem_st16(trow + C::COL_QLO + (d0 + i) / 2, lo);
                         }
                     }
                     tmem_wait_st();
+                    fence_proxy_async_smem();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars->q_full);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars->p_full[sb]);
-                pb = sb;
-                pph = sph;
-                if (++sb == NSB) {
-                    sb = 0;
-                    sph ^= 1u;
+                const float sl2 = p.scale_log2 * up;
+                for (uint32_t j = 0; j < nb; ++j) {
+                    const bool have = warp_wait_bounded(&bars->s_full[sb], sph, status, ST_PAGED_TIMEOUT, abort_flag);
+                    if (!work) {                             // no live row: P's lanes stay as they are, nothing reads them
+                        if (!named_bar_and(1 + qd, 64, have)) {
+                            ok = false;
+                            break;
+                        }
+                    } else {
+                        const uint32_t scol = trow + C::COL_S + sb * BN + h * HB;
+                        float sv[HB];
+                        if (have) {
+                            tc_fence_after();
+#pragma unroll
+                            for (int c = 0; c < HB / 32; ++c) {
+                                uint32_t rr[32];
+                                tmem_ld32(scol + c * 32, rr);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) sv[c * 32 + i] = __uint_as_float(rr[i]);
+                            }
+                            tmem_wait_ld();
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < HB; ++c) sv[c] = -INFINITY;
+                        }
+                        // causal mask; also drops the stale rows behind the last key (their S may be NaN)
+                        const int32_t kbase = static_cast<int32_t>((u.kb0 + j) * BN) + h * HB;
+                        if (static_cast<int32_t>((u.kb0 + j + 1) * BN) - 1 > qpos_min) {
+#pragma unroll
+                            for (int c = 0; c < HB; ++c)
+                                if (kbase + c > qpos) sv[c] = -INFINITY;
+                        }
+                        float mx4[4] = {sv[0], sv[1], sv[2], sv[3]};
+#pragma unroll
+                        for (int c = 4; c < HB; c += 4) {
+                            mx4[0] = fmaxf(mx4[0], sv[c]);
+                            mx4[1] = fmaxf(mx4[1], sv[c + 1]);
+                            mx4[2] = fmaxf(mx4[2], sv[c + 2]);
+                            mx4[3] = fmaxf(mx4[3], sv[c + 3]);
+                        }
+                        float* xb = xch + (j & 1) * (2 * BM);
+                        xb[h * BM + r] = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                        if (!named_bar_and(1 + qd, 64, have)) {
+                            ok = false;
+                            break;
+                        }
+                        const float mx = fmaxf(xb[r], xb[BM + r]) * sl2;
+                        const float m_new = fmaxf(m_run, mx);
+                        const bool grow = m_new > m_run + 8.0f;          // a stale m costs nothing up to 2^8
+                        const float m_use = grow ? m_new : m_run;
+                        const float alpha = grow ? ex2_approx(m_run - m_use) : 1.0f;
+                        const float m_sub = (m_use == -INFINITY ? 0.f : m_use) - kPUp;   // no key yet: p = 0
+                        const float2 sl2x2 = make_float2(sl2, sl2), negm = make_float2(-m_sub, -m_sub);
+                        const float2 neg1 = make_float2(-1.f, -1.f);
+                        float2 rs2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                        for (int c = 0; c < HB / 32; ++c) {   // 32 keys: 16 columns of P hi, then 16 of P lo
+                            uint32_t hi[16], lo[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) {
+                                const float2 x = __ffma2_rn(make_float2(sv[c * 32 + 2 * i], sv[c * 32 + 2 * i + 1]), sl2x2, negm);
+                                const float2 pp = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+                                rs2[i & 1] = __fadd2_rn(rs2[i & 1], pp);
+                                const __half2 hv = __floats2half2_rn(pp.x, pp.y);
+                                hi[i] = h2_bits(hv);
+                                if constexpr (PREC) {
+                                    const float2 d = __ffma2_rn(__half22float2(hv), neg1, pp);
+                                    lo[i] = h2_bits(__floats2half2_rn(d.x, d.y));
+                                }
+                            }
+                            tmem_st16(scol + c * 32, hi);
+                            if constexpr (PREC) tmem_st16(scol + c * 32 + 16, lo);
+                        }
+                        l_run = l_run * alpha + ((rs2[0].x + rs2[0].y) + (rs2[1].x + rs2[1].y));
+                        m_run = m_use;
+                        // ---- O rescale (rare) or fold (PREC), this half's columns: the last block's PV must have
+                        // finished.  Both halves of the rows see the same `grow`. ----
+                        const bool fold = PREC && j >= 1 && j % FOLD == 0;
+                        if (j >= 1 && (fold || __any_sync(0xffffffffu, grow))) {
+                            const bool done = warp_wait_bounded(&bars->pv_done[pb], pph, status, ST_PAGED_TIMEOUT, abort_flag);
+                            if (!named_bar_and(1 + qd, 64, done)) {
+                                ok = false;
+                                break;
+                            }
+                            tc_fence_after();
+                            const bool folded = PREC && j > FOLD;
+#pragma unroll 1
+                            for (int c = 0; c < HD / 2; c += 32) {
+                                float x[32];
+                                ld_o(c, x, fold && folded);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) x[i] *= alpha;
+                                if (fold) {
+                                    st_fold(c, x);
+                                    continue;
+                                }
+                                uint32_t rr[32];
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) rr[i] = __float_as_uint(x[i]);
+                                tmem_st32(ocol + c, rr);
+                                if constexpr (PREC) {
+                                    if (folded) {
+                                        ld_fold(c, x);
+#pragma unroll
+                                        for (int i = 0; i < 32; ++i) x[i] *= alpha;
+                                        st_fold(c, x);
+                                    }
+                                }
+                            }
+                        }
+                        tmem_wait_st();
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars->p_full[sb]);
+                    pb = sb;
+                    pph = sph;
+                    if (++sb == NSB) {
+                        sb = 0;
+                        sph ^= 1u;
+                    }
                 }
-            }
-            if (work) ld_gate(0, g);
-            // ---- the unit's rows: the slot that block nb-1 did not use is free (both halves have read it) ----
-            ok = ok && warp_wait_bounded(&bars->o_done, oph, status, ST_PAGED_TIMEOUT, abort_flag);
-            oph ^= 1u;
-            float* xl = xch + (nb & 1) * (2 * BM);
-            xl[h * BM + r] = l_run;
-            if (!named_bar_and(5, 256, ok)) break;       // every softmax warp
-            tc_fence_after();
-            l_row = xl[r] + xl[BM + r];
-            named_bar_sync(1 + qd, 64);                  // read before the next unit's Q maxima
+                if (work) ld_gate(0, g);
+                // ---- the unit's rows: the slot that block nb-1 did not use is free (both halves have read it) ----
+                ok = ok && warp_wait_bounded(&bars->o_done, oph, status, ST_PAGED_TIMEOUT, abort_flag);
+                oph ^= 1u;
+                float* xl = xch + (nb & 1) * (2 * BM);
+                xl[h * BM + r] = l_run;
+                if (!named_bar_and(5, 256, ok)) break;       // every softmax warp
+                tc_fence_after();
+                l_row = xl[r] + xl[BM + r];
+                named_bar_sync(1 + qd, 64);                  // read before the next unit's Q maxima
             } else if (work) {                           // no key to see: zeros
                 ld_gate(0, g);
             }
