@@ -249,8 +249,6 @@ def test_tiles_far_q(dev, act, scale):
     c.check()
 
 
-# ------------------------------------------------------- what the calls refuse or report
-
 def test_tiles_small_bf16_q_large_keys(dev):
     """bf16 q under fp16's normal range, halfway between two of its subnormals, against keys near fp16's largest: a
     plain conversion of q would be off by 2^-5 of it, scores of 0.67 by 0.02 and the outputs by 0.01."""
@@ -264,6 +262,70 @@ def test_tiles_small_bf16_q_large_keys(dev):
     c.run()
     c.check()
 
+
+def many_rows(H):
+    """Rows of q behind the last request that make a call large enough for two CTAs per SM (a tile per SM)."""
+    return -(-torch.cuda.get_device_properties(0).multi_processor_count * 128 // H)
+
+
+@pytest.mark.parametrize("act", ["f16", "bf16"])
+@pytest.mark.parametrize("H,KV,hd", [x for x in GEO if x[2] <= 128])
+@pytest.mark.parametrize("page,gate", [(16, False), (128, True), (256, False)])
+def test_large_calls_chunks(dev, act, H, KV, hd, page, gate):
+    """Two CTAs per SM: chunks of odd sizes, single tokens, requests without tokens or keys; padded rows stay."""
+    lens = [40, 1, 129, 700, 0, 65, 257, 300, 20]
+    new = [40, 1, 129, 33, 0, 1, 2, 100, 70]
+    c = Case(dev, H, KV, hd, page, lens, new, act=act, gate=gate, seed=H + hd + page, pad=many_rows(H),
+             stride_extra=16 if page == 128 else 0)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("act", ["f16", "bf16"])
+@pytest.mark.parametrize("lens,new", [
+    ([9], [9]), ([64], [64]), ([1000], [1000]), ([40000], [33]), ([17, 16, 15], [17, 16, 15]), ([3, 0, 40], [60, 20, 40]),
+    ([2500, 31, 1], [70, 31, 1]), ([1500, 900, 700], [700, 900, 65]),
+])
+@pytest.mark.parametrize("H,KV,hd", [(32, 8, 128), (14, 2, 64)])
+def test_large_calls_lengths(dev, act, lens, new, H, KV, hd):
+    c = Case(dev, H, KV, hd, 16, lens, new, act=act, seed=sum(lens) + hd, pad=many_rows(H))
+    c.run()
+    c.check()
+    first = c.out.clone()
+    for _ in range(3):
+        c.out.fill_(3.0)
+        c.run()
+        assert torch.equal(c.out, first)
+
+
+def test_large_calls_share_the_gpu(dev):
+    """Calls of every form in flight at once on streams of their own, eager and replayed."""
+    mk = lambda act, hd, pad, i: Case(dev, 8, 2, hd, 16, [3000 + 77 * i, 400], [300, 70], act=act, seed=50 + i, pad=pad)
+    cases = [mk("bf16", 128, many_rows(8), 0), mk("f16", 64, many_rows(8), 1), mk("f32", 128, 0, 2), mk("bf16", 256, 0, 3),
+             Case(dev, 32, 8, 128, 16, [20000], [1], seed=54)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for c, s in zip(cases, streams):
+        c.run(stream=s)
+    torch.cuda.synchronize()
+    graphs = []
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.run()
+        graphs.append(g)
+        c.out.fill_(3.0)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for c in cases:
+        c.check()
+
+
+# ------------------------------------------------------- what the calls refuse or report
 
 def test_bad_page_reads_as_zeros_and_is_reported(dev):
     """A block table entry outside the pool: status 602, and the other requests are untouched by it."""

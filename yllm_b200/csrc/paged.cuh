@@ -182,15 +182,17 @@ __device__ __forceinline__ long long div_pos(long long a, long long b) {
 
 // ROWS: query rows per tile (a row is one token x one head of the group); 0: a request's rows are one tile.
 // One warp runs it, all lanes.  Weights are in units of 1 / group key where ROWS, so that no sum needs a division.
-template <int BN, int ROWS> struct PagedSched {
+// PAIR: two CTAs share an SM and hide part of each other's fixed steps.  GATE_KEYS: charged for a unit whose output is
+// gated.
+template <int BN, int ROWS, bool PAIR = false, int GATE_KEYS = 0> struct PagedSched {
     // Keys charged for a unit besides its own, the least keys of a share where units are cut, the least blocks of a
     // cut unit's first and last piece.  A cut costs a partial's round trip through memory.  Decode form: about
     // 2.5 us, and a block 0.9 us when nothing else runs: shares of 128 beat 512 from 512 keys on (one Llama-3-8B
     // sequence, 1024 keys: 12.0 us against 17.6), and cutting a unit less than about fourfold loses (256 keys:
     // 12.0 us cut, 11.1 whole).
-    static constexpr long long kUnitCost = ROWS ? 512 : 192;
+    static constexpr long long kUnitCost = ROWS ? (PAIR ? 384 : 512) : 192;
     static constexpr long long kMinShare = ROWS ? 512 : 128;
-    static constexpr uint32_t kSnap = ROWS ? 256 / BN : 1;
+    static constexpr uint32_t kSnap = ROWS ? (PAIR ? 128 : 256) / BN : 1;
     static constexpr long long kCutFrom = ROWS ? 2 : 4;   // cut where a unit would get that many shares on average
     static_assert(kUnitCost >= BN && kMinShare >= BN, "a share inside a unit holds a block, so a cut unit's pieces are contiguous CTAs");
 
@@ -203,7 +205,12 @@ template <int BN, int ROWS> struct PagedSched {
 
     __device__ __forceinline__ explicit PagedSched(const PagedParams& pp) : p(pp) {}
 
-    static __device__ __forceinline__ long long unit_cost(const PagedParams& p) { return ROWS ? kUnitCost * p.group : kUnitCost; }
+    static __device__ __forceinline__ long long unit_keys(const PagedParams& p) {
+        return kUnitCost + (GATE_KEYS && p.gate ? GATE_KEYS : 0);
+    }
+    static __device__ __forceinline__ long long unit_cost(const PagedParams& p) {
+        return ROWS ? unit_keys(p) * p.group : kUnitCost;
+    }
     static __device__ __forceinline__ long long block_cost(const PagedParams& p) { return ROWS ? BN * static_cast<long long>(p.group) : BN; }
     static __device__ __forceinline__ uint32_t tiles(const PagedParams& p, const PagedReq& q) {
         if (!ROWS) return q.n > 0 ? 1u : 0u;
@@ -213,7 +220,7 @@ template <int BN, int ROWS> struct PagedSched {
     static __device__ __forceinline__ long long before(const PagedParams& p, const PagedReq& q, uint32_t t) {
         if (!ROWS) return t ? kUnitCost + q.len : 0;
         const long long T = t;
-        return T * ((kUnitCost + max(q.len - q.n, 0)) * p.group) + T * (T + 1) * (ROWS / 2);
+        return T * ((unit_keys(p) + max(q.len - q.n, 0)) * p.group) + T * (T + 1) * (ROWS / 2);
     }
     static __device__ __forceinline__ long long weight(const PagedParams& p, const PagedReq& q) {
         return before(p, q, tiles(p, q));

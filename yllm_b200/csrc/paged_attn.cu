@@ -11,7 +11,7 @@ namespace {
 size_t ml_offset() { return kPagedCounters * sizeof(uint32_t); }
 size_t workspace_bytes(uint32_t hd) {
     const size_t ctas = std::min<uint32_t>(static_cast<uint32_t>(dev_num_sms()), kPagedMaxPieces);
-    return ml_offset() + ctas * kPagedTileRows * (2 * 2 + 3 * static_cast<size_t>(hd)) * sizeof(float);
+    return ml_offset() + ctas * kPagedTileRows * (4 * 2 + 4 * static_cast<size_t>(hd)) * sizeof(float);
 }
 
 int attn_paged(void* out, uint32_t out_stride, const void* q, uint32_t q_stride, const void* gate,
@@ -116,7 +116,7 @@ int attn_paged(void* out, uint32_t out_stride, const void* q, uint32_t q_stride,
     p.counters = static_cast<uint32_t*>(ws);
     p.part_ml = reinterpret_cast<float*>(static_cast<char*>(ws) + ml_offset());
     p.part_o = p.part_ml + 2 * static_cast<size_t>(kPagedTileRows) *
-                               (2 * std::min<uint32_t>(static_cast<uint32_t>(dev_num_sms()), kPagedMaxPieces));
+                               (4 * std::min<uint32_t>(static_cast<uint32_t>(dev_num_sms()), kPagedMaxPieces));
     p.status = ctx->status;
     const uint64_t n_rows = static_cast<uint64_t>(n_pages) * page_size;
     // up to 8 query rows per kv head the warp-level kernel wastes no tensor work on absent rows; above, 128-row tiles

@@ -13,7 +13,7 @@
 // by 1.1e-5 without that, 2.6e-6 with sums of 1024 keys, 0.9e-6 with 256 (elementary fp32 operations: 1.3e-6),
 // for 1 % of the time at head_dim 128 and 15 % at 256, where the fold goes through global memory.
 //
-// One persistent CTA per SM walks its share of the schedule (paged.cuh).  Warps:
+// A persistent CTA, or a pair of them, per SM walks its share of the schedule (paged.cuh).  Alone, a CTA's warps:
 //   0-7  softmax: row r of the tile (TMEM lane r) belongs to warps r/32 and r/32 + 4, which halve each
 //        block's columns.  They fetch Q, turn S into P in place, rescale O when m grows by more than 2^8,
 //        and write the unit's rows or partials.  Rows are fetched and written through a warp's 2 KB of
@@ -22,6 +22,10 @@
 //   8, 10  K and V blocks by tensor copies into their rings, one copy per page and lane (4-D maps).
 //   9    MMA issue.  S runs up to NSB blocks ahead of the softmax.
 //   11   the schedule: units into a ring of four descriptors, so finding the next unit is off the others' path.
+// In a pair (16-bit activations, head_dim 64 and 128) a CTA has half of the SM's shared and tensor memory: blocks
+// of 64 keys, two S buffers at head_dim 128, four softmax warps with a whole row per thread, K, MMA, V and schedule
+// warps 4 to 7.  One CTA's Q, first S and rows out, and its waits for S, fall into the other's products and
+// exponentials: 785 cycles of the SM per 64 keys of a tile against 1,000.
 // V rows behind the last key the tile sees hold whatever the page held: the PV product stops at the 16-key
 // step that holds that key, and the rows after it in that step are zeroed in shared memory first.
 #include "paged.cuh"
@@ -34,16 +38,20 @@ namespace yattn {
 namespace {
 
 constexpr int BM = static_cast<int>(kPagedTileRows);
-constexpr int kTThreads = 384;
 constexpr int NU = 4;                    // unit descriptors in flight
-constexpr int kRegsSoftmax = 200, kRegsRest = 104;   // registers per thread after the split: 256 and 128 threads
 // P's factor: m may be stale by 8 binades, and fp16 ends below 2^16
 constexpr float kPUp = 7.f;
 
-template <int HD, bool PREC> struct TCfg {
-    static constexpr int BN = HD >= 256 ? 64 : 128;
+// PAIR: two CTAs per SM, 16-bit activations up to head_dim 128
+template <int HD, bool PREC, bool PAIR> struct TCfg {
+    static_assert(!PAIR || (!PREC && HD <= 128), "two CTAs' tensor and shared memory");
+    static constexpr int SPLIT = PAIR ? 1 : 2;              // threads per row
+    static constexpr int NSW = 4 * SPLIT, THREADS = 32 * (NSW + 4);
+    // registers per thread after the split
+    static constexpr int REGS_SOFTMAX = PAIR ? 168 : 200, REGS_REST = PAIR ? 88 : 104;
+    static constexpr int BN = HD >= 256 || PAIR ? 64 : 128;
     static constexpr bool LO_SMEM = PREC && HD <= 128;      // Q_lo in shared memory; head_dim 256: in TMEM
-    static constexpr int KST = HD >= 256 || (HD == 128 && PREC) ? 2 : 3;    // K ring depth
+    static constexpr int KST = HD >= 256 || (HD == 128 && (PREC || PAIR)) ? 2 : 3;    // K ring depth
     static constexpr int VST = HD >= 128 ? 2 : 3;           // V ring depth: V(j) is needed two blocks after K(j)
     static constexpr int Q_BYTES = BM * HD * 2;
     static constexpr int KV_BYTES = BN * HD * 2;
@@ -52,13 +60,13 @@ template <int HD, bool PREC> struct TCfg {
     static constexpr int OFF_K = OFF_QLO + (LO_SMEM ? Q_BYTES : 0);
     static constexpr int OFF_V = OFF_K + KST * KV_BYTES;
     static constexpr int OFF_STG = OFF_V + VST * KV_BYTES;  // per softmax warp: 32 rows x 64 B
-    static constexpr int OFF_X = OFF_STG + 8 * 2048;        // [2 blocks][2 halves][BM] floats: row maxima / sums
-    static constexpr int OFF_UP = OFF_X + 2 * 2 * BM * 4;   // [BM] floats: the rows' powers of two
+    static constexpr int OFF_X = OFF_STG + NSW * 2048;        // [2 blocks][2 halves][BM] floats: row maxima / sums
+    static constexpr int OFF_UP = OFF_X + (SPLIT - 1) * 2 * 2 * BM * 4;   // [BM] floats: the rows' powers of two
     static constexpr int OFF_U = OFF_UP + BM * 4;           // [NU] units, 64 B apart
     static constexpr int OFF_BAR = OFF_U + NU * 64;
     static constexpr int SMEM = OFF_BAR + 320 + 1024;       // + barriers, + alignment slack
-    static constexpr uint32_t TMEM_COLS = 512;
-    static constexpr int NSB = PREC ? 2 : 3;                // S buffers: b at columns [b*BN, (b+1)*BN)
+    static constexpr uint32_t TMEM_COLS = PAIR ? 256 : 512;
+    static constexpr int NSB = PREC || (PAIR && HD == 128) ? 2 : 3;                // S buffers: b at columns [b*BN, (b+1)*BN)
     static constexpr uint32_t COL_S = 0;
     static constexpr uint32_t COL_QLO = NSB * BN;           // head_dim 256, PREC: HD/2 columns
     static constexpr uint32_t COL_O = PREC ? 256 : NSB * BN;
@@ -68,7 +76,7 @@ template <int HD, bool PREC> struct TCfg {
     static constexpr uint32_t FOLD = 256 / BN;             // blocks per fold
     static_assert(COL_O + HD * (PREC && FOLD_TMEM ? 2 : 1) <= TMEM_COLS && NSB * BN <= static_cast<int>(COL_O), "TMEM columns");
     static_assert(!PREC || LO_SMEM || COL_QLO + HD / 2 <= COL_O, "Q_lo columns");
-    static_assert(SMEM <= 232448 && sizeof(PagedUnit) <= 64, "shared memory");
+    static_assert(SMEM <= (PAIR ? 115712 : 232448) && sizeof(PagedUnit) <= 64, "shared memory");
 };
 
 template <int KST, int VST> struct TBars {
@@ -116,15 +124,18 @@ __device__ __forceinline__ void stage_out(uint8_t* stg, int lane, const uint32_t
     __syncwarp();
 }
 
-template <int HD, int ACT>
-__global__ void __launch_bounds__(kTThreads, 1)
+template <int HD, int ACT, bool PAIR>
+__global__ void __launch_bounds__(TCfg<HD, ACT == YATTN_ACT_F32, PAIR>::THREADS, PAIR ? 2 : 1)
     k_paged_tiles(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                   const __grid_constant__ PagedParams p) {
     constexpr bool PREC = ACT == YATTN_ACT_F32;
-    using C = TCfg<HD, PREC>;
-    constexpr int BN = C::BN, HB = BN / 2, KST = C::KST, VST = C::VST, NPAN = HD / 64;
+    using C = TCfg<HD, PREC, PAIR>;
+    constexpr int NSW = C::NSW, SPLIT = C::SPLIT, HW = HD / SPLIT;   // softmax warps, threads per row, their columns of O
+    constexpr int BN = C::BN, HB = BN / SPLIT, KST = C::KST, VST = C::VST, NPAN = HD / 64;
     constexpr uint32_t NSB = C::NSB, FOLD = C::FOLD;
-    using Sched = PagedSched<BN, BM>;
+    // Charging 256 keys for the gate's way in: 8 gated chunks of the qwen3.5 shape 213 -> 200 us, of the Llama-3-8B shape
+    // 262 -> 246 (fp32 412 -> 386); at head_dim 64, with half the columns, it loses 3 %
+    using Sched = PagedSched<BN, BM, PAIR, HD >= 128 ? 256 : 0>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* sQ = smem + C::OFF_Q;
@@ -150,22 +161,22 @@ __global__ void __launch_bounds__(kTThreads, 1)
         }
         for (int s = 0; s < 3; ++s) {
             mbar_init(&bars->s_full[s], 1);
-            mbar_init(&bars->p_full[s], 8);
+            mbar_init(&bars->p_full[s], NSW);
             mbar_init(&bars->pv_done[s], 1);
         }
         mbar_init(&bars->o_done, 1);
-        mbar_init(&bars->q_full, 8);
+        mbar_init(&bars->q_full, NSW);
         mbar_init(&bars->mma_drain, 1);
         for (int s = 0; s < NU; ++s) {
             mbar_init(&bars->u_full[s], 1);
-            mbar_init(&bars->u_empty[s], 11);    // K, V, MMA and eight softmax warps
+            mbar_init(&bars->u_empty[s], 3 + NSW);    // K, V, MMA and the softmax warps
         }
         bars->abort_flag = 0;
         fence_mbar_init();
     }
     if (warp == 0) tmem_alloc(&bars->tmem_base, C::TMEM_COLS);
     Sched sched(p);                              // (its warp looks for the share meanwhile)
-    bool more = warp == 11 && sched.begin();
+    bool more = warp == NSW + 3 && sched.begin();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -182,9 +193,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
         if (lane == 0) mbar_arrive(&bars->u_empty[ui % NU]);
     };
     // registers move to the softmax warps (the launcher checks the sum against the launch's)
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
-        if (warp == 11) {
+    if (warp >= NSW) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_REST));
+        if (warp == NSW + 3) {
             // ================= schedule =================
             uint32_t ui = 0;
             bool ok = true;
@@ -216,9 +227,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 }
                 ++ui;
             }
-        } else if (warp == 8 || warp == 10) {
+        } else if (warp == NSW || warp == NSW + 2) {
             // ================= K / V copies =================
-            const bool is_v = warp == 10;
+            const bool is_v = warp == NSW + 2;
             const CUtensorMap* map = is_v ? &tmV : &tmK;
             uint8_t* ring = is_v ? sV : sK;
             uint64_t* full = is_v ? bars->v_full : bars->k_full;
@@ -385,9 +396,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
             __syncwarp();
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-        // ================= softmax warps 0-7 =================
-        const int qd = warp & 3, h = warp >> 2;          // TMEM lane quadrant, half of each block's columns
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SOFTMAX));
+        // ================= softmax warps =================
+        const int qd = warp & 3, h = warp >> 2;          // TMEM lane quadrant, half of each block's columns (SPLIT 1: 0)
         const int r = qd * 32 + lane;                    // row of the tile
         const uint32_t trow = tmem + (static_cast<uint32_t>(qd * 32) << 16);
         uint32_t sb = 0, sph = 0, pb = 0, pph = 0;       // S buffer of this block / of the last one, and parities
@@ -398,7 +409,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
         for (uint32_t ui = 0;; ++ui) {
             PagedUnit u;
             const bool got = get_unit(ui, u);
-            if (!named_bar_and(5, 256, got)) break;      // the end, or a wait that gave up
+            if (!named_bar_and(5, 32 * NSW, got)) break;      // the end, or a wait that gave up
             const uint32_t nb = u.kb1 - u.kb0;
             const uint32_t row0 = u.j * BM, rows = min(static_cast<uint32_t>(BM), static_cast<uint32_t>(u.n) * p.group - row0);
             const bool work = static_cast<uint32_t>(qd * 32) < rows;      // this warp has a live row
@@ -408,6 +419,8 @@ __global__ void __launch_bounds__(kTThreads, 1)
             const uint32_t hcol = (u.g * p.group + f - tk * p.group) * HD;
             const int32_t qpos = u.len - u.n + static_cast<int32_t>(tk);   // last key this row sees
             const int32_t qpos_min = u.len - u.n + static_cast<int32_t>(div_group(p, row0));
+            // the threads of these rows meet: the warp, or the two that halve the columns
+            auto rows_and = [&](bool x) -> bool { return SPLIT == 1 ? x : named_bar_and(1 + qd, 64, x); };
             // Columns [c, c + 32) of this half's rows, a row per lane, gated and rounded, out through the warp's
             // staging; g: their gate values from ld_gate(), in the staging's order.  All lanes.
             constexpr int ES = PREC ? 4 : 2, CW = 64 / ES, SUBS = 32 / CW;   // columns of a 64-byte run, runs
@@ -415,7 +428,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
             auto run_at = [&](int c, int i, size_t& token, size_t& col) -> bool {
                 const int rr = i * 8 + (lane >> 2);
                 token = static_cast<size_t>(u.tok0) + __shfl_sync(0xffffffffu, tk, rr);
-                col = __shfl_sync(0xffffffffu, hcol, rr) + static_cast<size_t>(h * (HD / 2) + c + (lane & 3) * (16 / ES));
+                col = __shfl_sync(0xffffffffu, hcol, rr) + static_cast<size_t>(h * HW + c + (lane & 3) * (16 / ES));
                 return static_cast<uint32_t>(qd * 32 + rr) < rows;
             };
             auto ld_gate = [&](int c, uint4 (&g)[SUBS * 4]) {
@@ -486,8 +499,8 @@ __global__ void __launch_bounds__(kTThreads, 1)
             uint4 g[SUBS * 4];                           // the gate of the next 32 columns, a step ahead
             bool ok = true;
             // ---- O and (PREC) the folded sum, 32 columns of this half at a time ----
-            const uint32_t ocol = trow + C::COL_O + h * (HD / 2), fcol = trow + C::COL_F + h * (HD / 2);
-            const int quad0 = h * (HD / 8);              // this half's first column quad
+            const uint32_t ocol = trow + C::COL_O + h * HW, fcol = trow + C::COL_F + h * HW;
+            const int quad0 = h * (HW / 4);              // this half's first column quad
             auto quads = [&](uint32_t slot) {            // partials by column quads: a warp's accesses are whole lines
                 return reinterpret_cast<float4*>(p.part_o) + (static_cast<size_t>(slot) * (HD / 4) + quad0) * BM + r;
             };
@@ -541,12 +554,12 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 float up = 1.f;
                 // ---- Q, each row scaled by its power of two: hi to shared memory, lo (PREC) beside it or to TMEM ----
                 if constexpr (!PREC || C::LO_SMEM) {
-                    // warp w fetches rows 16 w .. + 15, LPR lanes a row, 16 bytes a lane
-                    constexpr int ES = PREC ? 4 : 2, EL = 16 / ES, LPR = HD / EL, RPI = 32 / LPR, NI = 16 / RPI;
+                    // a warp fetches RPW rows, LPR lanes a row, 16 bytes a lane
+                    constexpr int ES = PREC ? 4 : 2, EL = 16 / ES, LPR = HD / EL, RPI = 32 / LPR, RPW = BM / NSW, NI = RPW / RPI;
                     uint4 raw[NI];
 #pragma unroll
                     for (int i = 0; i < NI; ++i) {
-                        const uint32_t row = warp * 16 + i * RPI + lane / LPR;
+                        const uint32_t row = warp * RPW + i * RPI + lane / LPR;
                         const uint32_t fr = row0 + min(row, rows - 1), tr = div_group(p, fr);
                         const size_t at = (static_cast<size_t>(u.tok0) + tr) * p.q_stride +
                                           (u.g * p.group + fr - tr * p.group) * HD + (lane % LPR) * EL;
@@ -585,14 +598,14 @@ __global__ void __launch_bounds__(kTThreads, 1)
                     if (plain) {
 #pragma unroll
                         for (int i = 0; i < NI; ++i) {
-                            const uint32_t row = warp * 16 + i * RPI + lane / LPR;
+                            const uint32_t row = warp * RPW + i * RPI + lane / LPR;
                             if (lane % LPR == 0) s_up[row] = 1.f;
                             *reinterpret_cast<uint4*>(sQ + sw128_offset(row, (lane % LPR) * EL, BM)) = raw[i];
                         }
                     } else {
 #pragma unroll
                         for (int i = 0; i < NI; ++i) {
-                            const uint32_t row = warp * 16 + i * RPI + lane / LPR;
+                            const uint32_t row = warp * RPW + i * RPI + lane / LPR;
                             const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
                             float x[EL], mx = 0.f;
 #pragma unroll
@@ -640,7 +653,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars->q_full);
-                    named_bar_sync(5, 256);                                   // s_up of every row
+                    named_bar_sync(5, 32 * NSW);                                   // s_up of every row
                     up = s_up[r];
                 } else {
                     // head_dim 256, fp32: a row's half per lane, in two passes (its largest value, then the planes)
@@ -703,7 +716,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 for (uint32_t j = 0; j < nb; ++j) {
                     const bool have = warp_wait_bounded(&bars->s_full[sb], sph, status, ST_PAGED_TIMEOUT, abort_flag);
                     if (!work) {                             // no live row: P's lanes stay as they are, nothing reads them
-                        if (!named_bar_and(1 + qd, 64, have)) {
+                        if (!rows_and(have)) {
                             ok = false;
                             break;
                         }
@@ -739,13 +752,15 @@ __global__ void __launch_bounds__(kTThreads, 1)
                             mx4[2] = fmaxf(mx4[2], sv[c + 2]);
                             mx4[3] = fmaxf(mx4[3], sv[c + 3]);
                         }
+                        float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
                         float* xb = xch + (j & 1) * (2 * BM);
-                        xb[h * BM + r] = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-                        if (!named_bar_and(1 + qd, 64, have)) {
+                        if constexpr (SPLIT == 2) xb[h * BM + r] = mx;
+                        if (!rows_and(have)) {
                             ok = false;
                             break;
                         }
-                        const float mx = fmaxf(xb[r], xb[BM + r]) * sl2;
+                        if constexpr (SPLIT == 2) mx = fmaxf(xb[r], xb[BM + r]);
+                        mx *= sl2;
                         const float m_new = fmaxf(m_run, mx);
                         const bool grow = m_new > m_run + 8.0f;          // a stale m costs nothing up to 2^8
                         const float m_use = grow ? m_new : m_run;
@@ -779,14 +794,14 @@ __global__ void __launch_bounds__(kTThreads, 1)
                         const bool fold = PREC && j >= 1 && j % FOLD == 0;
                         if (j >= 1 && (fold || __any_sync(0xffffffffu, grow))) {
                             const bool done = warp_wait_bounded(&bars->pv_done[pb], pph, status, ST_PAGED_TIMEOUT, abort_flag);
-                            if (!named_bar_and(1 + qd, 64, done)) {
+                            if (!rows_and(done)) {
                                 ok = false;
                                 break;
                             }
                             tc_fence_after();
                             const bool folded = PREC && j > FOLD;
 #pragma unroll 1
-                            for (int c = 0; c < HD / 2; c += 32) {
+                            for (int c = 0; c < HW; c += 32) {
                                 float x[32];
                                 ld_o(c, x, fold && folded);
 #pragma unroll
@@ -826,11 +841,14 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 ok = ok && warp_wait_bounded(&bars->o_done, oph, status, ST_PAGED_TIMEOUT, abort_flag);
                 oph ^= 1u;
                 float* xl = xch + (nb & 1) * (2 * BM);
-                xl[h * BM + r] = l_run;
-                if (!named_bar_and(5, 256, ok)) break;       // every softmax warp
+                if constexpr (SPLIT == 2) xl[h * BM + r] = l_run;
+                if (!named_bar_and(5, 32 * NSW, ok)) break;       // every softmax warp
                 tc_fence_after();
-                l_row = xl[r] + xl[BM + r];
-                named_bar_sync(1 + qd, 64);                  // read before the next unit's Q maxima
+                l_row = l_run;
+                if constexpr (SPLIT == 2) {
+                    l_row = xl[r] + xl[BM + r];
+                    named_bar_sync(1 + qd, 64);              // read before the next unit's Q maxima
+                }
             } else if (work) {                           // no key to see: zeros
                 ld_gate(0, g);
             }
@@ -847,7 +865,7 @@ __global__ void __launch_bounds__(kTThreads, 1)
                 if (work) {
                     float4* po = quads(u.slot);
 #pragma unroll 1
-                    for (int c = 0; c < HD / 2; c += 32) {
+                    for (int c = 0; c < HW; c += 32) {
                         float x[32];
                         ld_o(c, x, folded);
 #pragma unroll
@@ -856,10 +874,10 @@ __global__ void __launch_bounds__(kTThreads, 1)
                     }
                 }
                 __threadfence();
-                named_bar_sync(5, 256);
+                named_bar_sync(5, 32 * NSW);
                 if (threadIdx.x == 0)
                     bars->last_flag = atomicInc(&p.counters[u.c_first], u.n_pieces - 1) == u.n_pieces - 1;
-                named_bar_sync(5, 256);
+                named_bar_sync(5, 32 * NSW);
                 write = bars->last_flag && work;
                 if (write) {
                     __threadfence();
@@ -876,9 +894,9 @@ __global__ void __launch_bounds__(kTThreads, 1)
             }
             if (write) {
 #pragma unroll 1
-                for (int c = 0; c < HD / 2; c += 32) {
+                for (int c = 0; c < HW; c += 32) {
                     uint4 g_next[SUBS * 4];
-                    if (c + 32 < HD / 2) ld_gate(c + 32, g_next);
+                    if (c + 32 < HW) ld_gate(c + 32, g_next);
                     float x[32];
                     if (u.n_pieces > 1) {                // in piece order
 #pragma unroll
@@ -928,29 +946,29 @@ __global__ void __launch_bounds__(kTThreads, 1)
     if (warp == 0) tmem_dealloc(tmem, C::TMEM_COLS);
 }
 
-template <int HD, int ACT>
+template <int HD, int ACT, bool PAIR>
 int launch(const PagedParams& p, const CUtensorMap& mk, const CUtensorMap& mv, uint32_t ctas, cudaStream_t st,
            char* err, size_t errlen) {
-    using C = TCfg<HD, ACT == YATTN_ACT_F32>;
+    using C = TCfg<HD, ACT == YATTN_ACT_F32, PAIR>;
     static bool attr_done[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev >= 0 && dev < 64 && !attr_done[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(k_paged_tiles<HD, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(k_paged_tiles<HD, ACT, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) {
             set_err(err, errlen, "attn_paged: smem attribute (%d bytes): %s", C::SMEM, cudaGetErrorString(e));
             return -1;
         }
         // an increase past what the block was launched with would wait for ever
         cudaFuncAttributes at{};
-        e = cudaFuncGetAttributes(&at, k_paged_tiles<HD, ACT>);
-        if (e != cudaSuccess || at.numRegs * kTThreads < 256 * kRegsSoftmax + 128 * kRegsRest) {
+        e = cudaFuncGetAttributes(&at, k_paged_tiles<HD, ACT, PAIR>);
+        if (e != cudaSuccess || at.numRegs * C::THREADS < 32 * C::NSW * C::REGS_SOFTMAX + 128 * C::REGS_REST) {
             set_err(err, errlen, "attn_paged: built with %d registers a thread, too few for the register split", at.numRegs);
             return -1;
         }
         attr_done[dev] = true;
     }
-    k_paged_tiles<HD, ACT><<<ctas, kTThreads, C::SMEM, st>>>(mk, mv, p);
+    k_paged_tiles<HD, ACT, PAIR><<<ctas * (PAIR ? 2 : 1), C::THREADS, C::SMEM, st>>>(mk, mv, p);
     YATTN_CHECK_LAUNCH(err, errlen, "attn_paged");
     return 0;
 }
@@ -962,18 +980,28 @@ int paged_tiles(const PagedParams& pp, const uint16_t* kpool, const uint16_t* vp
     PagedParams p = pp;
     p.hc = 1;
     p.n_groups = n_kv;
-    const uint32_t bn = hd >= 256 ? 64 : 128, box = std::min(1u << p.page_shift, bn);
+    const uint32_t sms = static_cast<uint32_t>(dev_num_sms());
+    // Two CTAs per SM from a tile per SM on: below that most SMs would hold one of them, slower than a CTA that has
+    // the SM to itself (bf16, Llama-3-8B: 4096-token prompt 177 us against 197, 300 tokens behind 700: 31 against 27)
+    const bool pair = hd <= 128 && p.act != YATTN_ACT_F32 &&
+                      static_cast<uint64_t>(p.n_tokens) * p.n_heads >= static_cast<uint64_t>(sms) * kPagedTileRows;
+    const uint32_t bn = hd >= 256 || pair ? 64 : 128, box = std::min(1u << p.page_shift, bn);
     CUtensorMap mk, mv;
     if (encode_page_map(&mk, kpool, kv_dim, n_rows, n_kv * hd, box, hd / 64, err, errlen) ||
         encode_page_map(&mv, vpool, kv_dim, n_rows, n_kv * hd, box, hd / 64, err, errlen))
         return -1;
-    const uint32_t ctas = std::min<uint32_t>(static_cast<uint32_t>(dev_num_sms()), kPagedMaxPieces);
+    const uint32_t ctas = std::min<uint32_t>(sms, kPagedMaxPieces);
     auto run = [&](auto tag) -> int {
         constexpr int HD = decltype(tag)::value;
+        if constexpr (HD <= 128) {
+            if (pair)
+                return p.act == YATTN_ACT_F16 ? launch<HD, YATTN_ACT_F16, true>(p, mk, mv, ctas, st, err, errlen)
+                                              : launch<HD, YATTN_ACT_BF16, true>(p, mk, mv, ctas, st, err, errlen);
+        }
         switch (p.act) {
-            case YATTN_ACT_F32: return launch<HD, YATTN_ACT_F32>(p, mk, mv, ctas, st, err, errlen);
-            case YATTN_ACT_F16: return launch<HD, YATTN_ACT_F16>(p, mk, mv, ctas, st, err, errlen);
-            default: return launch<HD, YATTN_ACT_BF16>(p, mk, mv, ctas, st, err, errlen);
+            case YATTN_ACT_F32: return launch<HD, YATTN_ACT_F32, false>(p, mk, mv, ctas, st, err, errlen);
+            case YATTN_ACT_F16: return launch<HD, YATTN_ACT_F16, false>(p, mk, mv, ctas, st, err, errlen);
+            default: return launch<HD, YATTN_ACT_BF16, false>(p, mk, mv, ctas, st, err, errlen);
         }
     };
     switch (hd) {
