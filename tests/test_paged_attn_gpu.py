@@ -263,6 +263,19 @@ def test_tiles_small_bf16_q_large_keys(dev):
     c.check()
 
 
+@pytest.mark.parametrize("H,KV,hd", [(8, 2, 128), (3, 3, 64), (14, 2, 64), (32, 2, 128)])
+@pytest.mark.parametrize("gate", [False, True])
+def test_few_rows_beside_many(dev, H, KV, hd, gate):
+    """fp32 requests around half a tile of query rows, whole and cut over many CTAs, with rows that see no key and with
+    q far outside fp16's range."""
+    g = H // KV
+    new = [64 // g, 64 // g + 1, 1, 64 // g - 1, 0, 65, 64 // g, 2, 9]
+    lens = [64 // g, 700, 130, 3 * 128, 50, 300, 9000, 1, 20001]
+    c = Case(dev, H, KV, hd, 16, lens, new, gate=gate, seed=H + hd, pad=2, q_scale=2.0 ** -20 if gate else 1.0)
+    c.run(max_new=128)
+    c.check(max_new=128)
+
+
 def many_rows(H):
     """Rows of q behind the last request that make a call large enough for two CTAs per SM (a tile per SM)."""
     return -(-torch.cuda.get_device_properties(0).multi_processor_count * 128 // H)
