@@ -251,6 +251,14 @@ def test_store(dev, act, H, KV, hd, kind, n_dims, theta, norm, T, pad, fused):
     assert (rows_k[:, KV * hd:] == 0x7BCD).all() and (rows_v[:, KV * hd:] == 0x7BCD).all()
 
 
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("T", [1500, 3001, 5003])
+@pytest.mark.parametrize("H,KV,hd,kind,n_dims,norm", [(16, 8, 128, 1, 0, "f32"), (16, 2, 256, 2, 64, None), (16, 8, 128, 0, 0, None)])
+def test_store_many_tokens(dev, act, T, H, KV, hd, kind, n_dims, norm):
+    """Several tokens a block, one, two and four of them per barrier, the last ones of a group missing or skipped."""
+    test_store(dev, act, H, KV, hd, kind, n_dims, 1e6, norm, T, 7, True)
+
+
 def test_store_in_place_and_bad_slot(dev):
     """q_out = q; a slot outside the pool stores nothing and is reported."""
     from yllm_b200 import attn
