@@ -569,8 +569,10 @@ int yattn_rope_store_kv_paged(void* q_out, uint32_t q_out_stride, const void* q,
  * apart.  Rows from cu_new[n_seqs] on are not written; n_tokens is q's row
  * count.  max_new is an upper bound of the requests' new tokens (host): up to 8
  * query rows per kv head (max_new * n_heads/n_kv_heads) run the decode form,
- * more run 128-row tiles on tcgen05.  Work is divided evenly over the SMs from
- * the lengths on the device, so nothing here depends on them at capture time.
+ * more run 128-row tiles on tcgen05; an fp32 batch of mostly such small requests
+ * (n_seqs * n_kv_heads >= SMs, 4 n_tokens <= n_seqs * max_new) runs both, a launch
+ * each.  Work is divided evenly over the SMs from the lengths on the device, so
+ * nothing here depends on them at capture time.
  * fp32 activations keep about 22 bits of q and of the softmax weights (fp16 hi
  * + lo planes); 16-bit activations run one plane of each in the tiles form
  * (bf16 q to 2^-19 or better of its row's largest).

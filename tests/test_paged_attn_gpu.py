@@ -276,6 +276,59 @@ def test_few_rows_beside_many(dev, H, KV, hd, gate):
     c.check(max_new=128)
 
 
+@pytest.mark.parametrize("H,KV,hd,gate", [(14, 2, 64, False), (32, 8, 128, True), (16, 2, 256, False), (5, 5, 64, True)])
+@pytest.mark.parametrize("page", [16, 128])
+def test_mixed_batch_in_two_launches(dev, H, KV, hd, gate, page):
+    """fp32, as many requests as make a kv head of one per SM: single tokens and small requests around 8 query rows
+    per kv head beside chunks, requests without tokens, without keys, and with fewer keys than tokens."""
+    rng = np.random.default_rng(H + page)
+    n = -(-torch.cuda.get_device_properties(0).multi_processor_count // KV) + 3
+    few = 8 // (H // KV)
+    new = rng.choice([0, 1, 1, 1, 1, max(few, 1), few + 1], n)
+    new[[1, n // 2]] = 150, 333
+    lens = new + rng.integers(0, 700, n)
+    lens[[0, 2, 5]] = 0, new[2], max(int(new[5]) - 1, 0)
+    lens[1] = 100
+    assert int(new.sum()) * 4 <= n * 333
+    c = Case(dev, H, KV, hd, page, lens, new, gate=gate, seed=H + hd + page, pad=2)
+    c.run()
+    c.check()
+    first = c.out.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        c.run()
+    for _ in range(3):
+        c.out.fill_(3.0)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(c.out, first)
+
+
+def test_mixed_batch_in_two_launches_skips_a_bad_request(dev):
+    """A request longer than its table: reported, its rows not written, the others right."""
+    from yllm_b200 import attn
+    n = torch.cuda.get_device_properties(0).multi_processor_count
+    new = [1] * n
+    new[7], new[20] = 200, 60
+    lens = [100 + i for i in range(n)]
+    lens[7] = 300
+    c = Case(dev, 8, 2, 128, 16, lens, new, seed=77)
+    at = np.concatenate([[0], np.cumsum(new)])
+    for bad in (3, 20):
+        c.kv[bad] = c.tables.shape[1] * 16 + 1
+    c.run()
+    torch.cuda.synchronize()
+    assert attn.device_status() == 603
+    want, bar = c.want(False)
+    err = (c.out[:c.total, :1024].double() - want).abs()
+    for r in range(n):
+        part = slice(at[r], at[r + 1])
+        if r in (3, 20):
+            assert bool((c.out[part] == 3.0).all())
+        else:
+            assert bool((err[part] <= bar[part]).all()), r
+
+
 def many_rows(H):
     """Rows of q behind the last request that make a call large enough for two CTAs per SM (a tile per SM)."""
     return -(-torch.cuda.get_device_properties(0).multi_processor_count * 128 // H)

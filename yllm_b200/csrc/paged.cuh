@@ -29,6 +29,7 @@ struct PagedParams {
     uint32_t table_stride, max_pages, n_pages, page_shift;
     uint32_t n_tokens, n_seqs, max_new;
     uint32_t n_heads, group;          // query heads, query heads per kv head
+    uint32_t rows_lo, rows_hi;        // requests of rows_lo to rows_hi query rows per kv head are this launch's
     uint32_t group_m, group_s;        // x / group = x * group_m >> group_s for x < 2^31
     uint32_t hc, n_groups;            // kv heads per unit, units' head groups (n_kv / hc)
     int act;                          // YATTN_ACT_*
@@ -150,6 +151,8 @@ __device__ __forceinline__ PagedReq paged_req(const PagedParams& p, uint32_t r) 
         atomicCAS(p.status, 0, ST_PAGED_BAD_REQUEST);
         q.tok0 = q.n = q.len = 0;
     }
+    const uint32_t rows = static_cast<uint32_t>(q.n) * p.group;
+    if (rows < p.rows_lo || rows > p.rows_hi) q.n = 0;
     return q;
 }
 
