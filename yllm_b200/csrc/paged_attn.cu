@@ -126,7 +126,7 @@ int attn_paged(void* out, uint32_t out_stride, const void* q, uint32_t q_stride,
     // Many requests, most of them of far fewer tokens than the largest: with fp32 activations, whose tiles take four
     // products, those that fit the warp-level kernel go there in a second launch.  From a request's kv head per SM on;
     // the launch costs 8 to 10 us where it finds less (Llama-3-8B shape: 28 single tokens beside 4 chunks 352 -> 314 us,
-    // 63 beside one 186 -> 150, but 14 beside 2 76 -> 85)
+    // 63 beside one 186 -> 150, but 14 beside 2 76 -> 85).  With 16-bit activations it mostly loses: bf16 221 -> 238
     const bool split = act == YATTN_ACT_F32 && p.group <= kPagedRows &&
                        static_cast<uint64_t>(n_seqs) * n_kv >= static_cast<uint64_t>(ctx->num_sms) &&
                        static_cast<uint64_t>(n_tokens) * 4 <= static_cast<uint64_t>(n_seqs) * p.max_new;
