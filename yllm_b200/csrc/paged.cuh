@@ -36,7 +36,7 @@ struct PagedParams {
     float scale_log2;                 // log2(e) / sqrt(head_dim)
     uint32_t* counters;               // [gridDim.x]: pieces of a cut unit that are done, by its first CTA
     float* part_ml;                   // [2 * gridDim.x][rows][2]
-    float* part_o;                    // [3 * gridDim.x][rows][HD]: two partials a CTA, then a folded sum each
+    float* part_o;                    // [2 * gridDim.x][rows][HD]: two partials a CTA (tiles: or a folded sum in the second)
     int* status;
 };
 

@@ -6,8 +6,8 @@
 namespace yattn {
 namespace {
 
-// Workspace: kPagedCounters counters (zero between calls), then the partial rows' (m, l), two slots per CTA, and
-// o, two slots per CTA and one for the folded sums.  The tiles kernel's slots are the larger ones.
+// Workspace: kPagedCounters counters (zero between calls), then the partial rows' (m, l) and o, two slots per CTA and
+// two CTAs per SM.  The tiles kernel's slots are the larger ones.
 size_t ml_offset() { return kPagedCounters * sizeof(uint32_t); }
 size_t workspace_bytes(uint32_t hd) {
     const size_t ctas = std::min<uint32_t>(static_cast<uint32_t>(dev_num_sms()), kPagedMaxPieces);

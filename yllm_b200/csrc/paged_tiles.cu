@@ -11,7 +11,9 @@
 // it adds to an accumulator, always towards zero, so PREC issues Q_lo K before Q_hi K, sums at most 256 keys
 // of P V in one accumulator and adds those sums in fp32 (the fold below).  Over 8700 keys the result was off
 // by 1.1e-5 without that, 2.6e-6 with sums of 1024 keys, 0.9e-6 with 256 (elementary fp32 operations: 1.3e-6),
-// for 1 % of the time at head_dim 128 and 15 % at 256, where the fold goes through global memory.
+// for 1 % of the time at head_dim 128 and 15 % at 256, where the fold goes through global memory.  16-bit
+// activations sum 8192 keys, through global memory too: the drift stays under 2^-14 of the result, far below its
+// rounding.  With one accumulator it was 2.3e-4 over 131,072 keys and 4e-3 over 2^20.
 //
 // A persistent CTA, or a pair of them, per SM walks its share of the schedule (paged.cuh).  Alone, a CTA's warps:
 //   0-7  softmax: row r of the tile (TMEM lane r) belongs to warps r/32 and r/32 + 4, which halve each
@@ -70,11 +72,11 @@ template <int HD, bool PREC, bool PAIR> struct TCfg {
     static constexpr uint32_t COL_S = 0;
     static constexpr uint32_t COL_QLO = NSB * BN;           // head_dim 256, PREC: HD/2 columns
     static constexpr uint32_t COL_O = PREC ? 256 : NSB * BN;
-    // PREC: the fp32 sum of the folded O.  Beside O, or at head_dim 256, where TMEM is full, in global memory
-    static constexpr bool FOLD_TMEM = HD <= 128;
+    // The fp32 sum of the folded O: beside O, or where TMEM is full (16 bits, head_dim 256) in global memory
+    static constexpr bool FOLD_TMEM = PREC && HD <= 128;
     static constexpr uint32_t COL_F = COL_O + HD;
-    static constexpr uint32_t FOLD = 256 / BN;             // blocks per fold
-    static_assert(COL_O + HD * (PREC && FOLD_TMEM ? 2 : 1) <= TMEM_COLS && NSB * BN <= static_cast<int>(COL_O), "TMEM columns");
+    static constexpr uint32_t FOLD = (PREC ? 256 : 8192) / BN;             // blocks per fold
+    static_assert(COL_O + HD * (FOLD_TMEM ? 2 : 1) <= TMEM_COLS && NSB * BN <= static_cast<int>(COL_O), "TMEM columns");
     static_assert(!PREC || LO_SMEM || COL_QLO + HD / 2 <= COL_O, "Q_lo columns");
     static_assert(SMEM <= (PAIR ? 115712 : 232448) && sizeof(PagedUnit) <= 64, "shared memory");
 };
@@ -356,7 +358,7 @@ __global__ void __launch_bounds__(TCfg<HD, ACT == YATTN_ACT_F32, PAIR>::THREADS,
                     const uint32_t pcol = tmem + C::COL_S + warp_uniform(pv_sb * BN);
                     const uint64_t dv = dv0 + warp_uniform((vs * C::KV_BYTES) >> 4);
                     if (elect_one()) {
-                        const bool fresh = PREC ? jj % FOLD == 0 : jj == 0;   // PREC: the sum so far has been folded
+                        const bool fresh = jj % FOLD == 0;                    // the sum so far has been folded
 #pragma unroll
                         for (int plane = 0; plane < (PREC ? 2 : 1); ++plane)
 #pragma unroll
@@ -494,17 +496,18 @@ __global__ void __launch_bounds__(TCfg<HD, ACT == YATTN_ACT_F32, PAIR>::THREADS,
                     }
                 }
             };
-            const bool folded = PREC && nb > FOLD;
+            const bool folded = nb > FOLD;
             float m_run = -INFINITY, l_run = 0.f, l_row = 0.f;   // log2 units; l_run: this half's columns
             uint4 g[SUBS * 4];                           // the gate of the next 32 columns, a step ahead
             bool ok = true;
-            // ---- O and (PREC) the folded sum, 32 columns of this half at a time ----
+            // ---- O and the folded sum, 32 columns of this half at a time ----
             const uint32_t ocol = trow + C::COL_O + h * HW, fcol = trow + C::COL_F + h * HW;
             const int quad0 = h * (HW / 4);              // this half's first column quad
             auto quads = [&](uint32_t slot) {            // partials by column quads: a warp's accesses are whole lines
                 return reinterpret_cast<float4*>(p.part_o) + (static_cast<size_t>(slot) * (HD / 4) + quad0) * BM + r;
             };
-            float4* const fsum = quads(2 * gridDim.x + blockIdx.x);
+            // (the slot of the piece that ends this CTA's share: the last one to be written, from these very sums)
+            float4* const fsum = quads(2 * blockIdx.x + 1);
             auto ld_fold = [&](int c, float (&x)[32]) {
                 if constexpr (C::FOLD_TMEM) {
                     uint32_t rr[32];
@@ -541,13 +544,11 @@ __global__ void __launch_bounds__(TCfg<HD, ACT == YATTN_ACT_F32, PAIR>::THREADS,
                 tmem_wait_ld();
 #pragma unroll
                 for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(rr[i]);
-                if constexpr (PREC) {
-                    if (folded) {
-                        float y[32];
-                        ld_fold(c, y);
+                if (folded) {
+                    float y[32];
+                    ld_fold(c, y);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] += y[i];
-                    }
+                    for (int i = 0; i < 32; ++i) x[i] += y[i];
                 }
             };
             if (nb > 0) {
@@ -789,9 +790,9 @@ __global__ void __launch_bounds__(TCfg<HD, ACT == YATTN_ACT_F32, PAIR>::THREADS,
                         }
                         l_run = l_run * alpha + ((rs2[0].x + rs2[0].y) + (rs2[1].x + rs2[1].y));
                         m_run = m_use;
-                        // ---- O rescale (rare) or fold (PREC), this half's columns: the last block's PV must have
+                        // ---- O rescale (rare) or fold, this half's columns: the last block's PV must have
                         // finished.  Both halves of the rows see the same `grow`. ----
-                        const bool fold = PREC && j >= 1 && j % FOLD == 0;
+                        const bool fold = j >= 1 && j % FOLD == 0;
                         if (j >= 1 && (fold || __any_sync(0xffffffffu, grow))) {
                             const bool done = warp_wait_bounded(&bars->pv_done[pb], pph, status, ST_PAGED_TIMEOUT, abort_flag);
                             if (!rows_and(done)) {
@@ -799,7 +800,7 @@ __global__ void __launch_bounds__(TCfg<HD, ACT == YATTN_ACT_F32, PAIR>::THREADS,
                                 break;
                             }
                             tc_fence_after();
-                            const bool folded = PREC && j > FOLD;
+                            const bool folded = j > FOLD;
 #pragma unroll 1
                             for (int c = 0; c < HW; c += 32) {
                                 float x[32];
@@ -814,13 +815,11 @@ __global__ void __launch_bounds__(TCfg<HD, ACT == YATTN_ACT_F32, PAIR>::THREADS,
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) rr[i] = __float_as_uint(x[i]);
                                 tmem_st32(ocol + c, rr);
-                                if constexpr (PREC) {
-                                    if (folded) {
-                                        ld_fold(c, x);
+                                if (folded) {
+                                    ld_fold(c, x);
 #pragma unroll
-                                        for (int i = 0; i < 32; ++i) x[i] *= alpha;
-                                        st_fold(c, x);
-                                    }
+                                    for (int i = 0; i < 32; ++i) x[i] *= alpha;
+                                    st_fold(c, x);
                                 }
                             }
                         }
