@@ -20,6 +20,7 @@
 #include "common.cuh"
 
 #include <algorithm>
+#include <atomic>
 
 namespace yattn {
 namespace {
@@ -269,13 +270,17 @@ extern "C" int yattn_page_step(int32_t* kv_len_out, int32_t* cu_new, int32_t* sl
     p.page_shift = static_cast<uint32_t>(__builtin_ctz(page_size));
     p.status = ctx->status;
     const size_t smem = 3 * (static_cast<size_t>(n_seqs) + 1) * 4;
-    if (smem > 48 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(k_page_step, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(smem));
+    // the limit is the kernel's, not the call's: raised once to what the largest call needs, so that no other thread's
+    // call finds it lower than its own size
+    static std::atomic<bool> attr_done[64];
+    if (!attr_done[ctx->device].load(std::memory_order_acquire)) {
+        constexpr int kMaxSmem = 3 * (static_cast<int>(kMaxSeqs) + 1) * 4;
+        cudaError_t e = cudaFuncSetAttribute(k_page_step, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
         if (e != cudaSuccess) {
-            set_err(err, errlen, "page_step: smem attribute (%zu bytes): %s", smem, cudaGetErrorString(e));
+            set_err(err, errlen, "page_step: smem attribute (%d bytes): %s", kMaxSmem, cudaGetErrorString(e));
             return -1;
         }
+        attr_done[ctx->device].store(true, std::memory_order_release);
     }
     // a token a thread up to one block per SM; the prefix sums are repeated in every block
     const uint32_t work = std::max(max_tokens, n_seqs + 1);
