@@ -548,7 +548,9 @@ int yattn_page_step(int32_t* kv_len_out, int32_t* cu_new, int32_t* slots, int32_
  * rope_kind, n_rope_dims (kind 2: a multiple of 16) and qk_norm as
  * yattn_rope_store_kv, but the angle position*theta^(-2j/n) is taken in 64
  * bits (that call's fp32 angle drifts by half an ulp of itself at far
- * positions).  head_dim 64/128/256.  q, k, v, q_out and the pools are 16-byte
+ * positions).  A head of finite values whose sum of squares passes fp32 is
+ * normalised to zeros.
+ * head_dim 64/128/256.  q, k, v, q_out and the pools are 16-byte
  * aligned, strides multiples of 16 bytes, kv_dim a multiple of 8. */
 int yattn_rope_store_kv_paged(void* q_out, uint32_t q_out_stride, const void* q, uint32_t q_stride,
                               const void* k, uint32_t k_stride, const void* v, uint32_t v_stride, int act,

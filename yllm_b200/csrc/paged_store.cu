@@ -176,14 +176,16 @@ __global__ void __launch_bounds__(512, sizeof(T) == 4 ? 3 : 2) k_paged_store(con
             if (!is_v) {
                 const float m = ss * (1.0f / HD) + p.eps;
                 float inv = rsqrtf(m);
-                inv = inv * (1.5f - 0.5f * m * inv * inv);   // one Newton step: rsqrt.approx is 2 ulp off
+                // one Newton step: rsqrt.approx is 2 ulp off.  Where the squares passed fp32, 1 / sqrt(m) = 0 stays, and
+                // x goes times it before w: x w may pass fp32 as well
+                inv = m < INFINITY ? inv * (1.5f - 0.5f * m * inv * inv) : inv;
                 float wa[VEC], wb[VEC];
                 lds(s_w[is_q ? 0 : 1] + ea, wa);
                 lds(s_w[is_q ? 0 : 1] + eb, wb);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    a[i] = a[i] * wa[i] * inv;
-                    b[i] = b[i] * wb[i] * inv;
+                    a[i] = a[i] * inv * wa[i];
+                    b[i] = b[i] * inv * wb[i];
                 }
             }
         }
