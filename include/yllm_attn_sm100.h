@@ -528,6 +528,11 @@ enum { YATTN_ACT_F32 = 0, YATTN_ACT_F16 = 1, YATTN_ACT_BF16 = 2 };   /* activati
  * kv_len, cu_new is all zero and every slot -1 (so the calls that read them do
  * nothing): > 0 = pages missing, -1 = more than max_tokens tokens, -2 = a
  * request needs more than max_pages pages, -3 = malformed lengths or queue.
+ * The page numbers themselves do not decide the verdict: a number outside the
+ * pool, in the queue or in a table, moves as any other does, and every step that
+ * hands one out to a token, returns one or puts a token into one sets device
+ * status 602 (the token's slot is -1).  Such a number stays in the queue, so
+ * after a 602 from this call tables and ring have to be set up anew.
  * The inputs kv_len, new_len and state stay as they are and must not overlap
  * the outputs: feed kv_len_out and state_out to the next step (two sets of
  * buffers in turn).  state_out is 16-byte aligned.  1 to 16384 requests. */
