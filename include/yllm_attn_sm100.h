@@ -592,7 +592,8 @@ int yattn_rope_store_kv_paged(void* q_out, uint32_t q_out_stride, const void* q,
  * head_dim 64/128/256, n_heads a multiple of n_kv_heads; out overlaps nothing.
  * workspace: yattn_attn_paged_workspace_bytes, its first 4096 bytes zeroed once; a
  * call leaves them zero.  Calls that may overlap (other streams, graphs) need
- * a workspace each; after status 601 zero it again. */
+ * a workspace each.  After a call that gave up (601) zero it again; the status
+ * word keeps the first code only, so do that after any other code too. */
 size_t yattn_attn_paged_workspace_bytes(uint32_t head_dim);
 int yattn_attn_paged(void* out, uint32_t out_stride, const void* q, uint32_t q_stride, const void* gate,
                      uint32_t gate_stride, int act, const uint16_t* kpool, const uint16_t* vpool,

@@ -608,8 +608,10 @@ def sess_kv_load(kv: torch.Tensor, n_blocks: int, kv_dim: int, max_seq: int, pat
 def device_status(clear: bool = True) -> int:
     st = C.c_int(0)
     call("yattn_device_status", C.byref(st), 1 if clear else 0)
-    if st.value == 601:
-        _paged_ws.clear()   # a paged attention gave up: its workspace's counters are not zero any more
+    if st.value != 0:
+        # a paged attention that gave up (601) leaves its workspace's counters other than zero.  The word holds the first
+        # code only, so any code may stand before a 601
+        _paged_ws.clear()
     return st.value
 
 
