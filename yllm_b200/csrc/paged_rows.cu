@@ -354,8 +354,8 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
         const bool whole = u.n_pieces == 1;
         // one warp per (kv head, query row)
         auto finish = [&](uint32_t h, uint32_t f, const float (&acc)[DPL], float l) {
-            const float inv = l == 0.f ? 0.f : 1.0f / l;      // no key seen: zeros
             const uint32_t tk = f / p.group;
+            const float inv = u.len - u.n + static_cast<int32_t>(tk) < 0 ? 0.f : 1.0f / l;   // no key seen: zeros
             const size_t tok = u.tok0 + static_cast<size_t>(tk);
             const size_t col = static_cast<size_t>((u.g * HC + h) * p.group + f - tk * p.group) * HD + lane * DPL;
             float x[DPL];

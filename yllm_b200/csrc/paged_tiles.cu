@@ -853,7 +853,9 @@ __global__ void __launch_bounds__(TCfg<HD, ACT == YATTN_ACT_F32, PAIR>::THREADS,
             }
             // ---- the unit's rows, or a piece's (m, l, o) and, of the last piece to arrive, the merged rows ----
             bool write = work;
-            float M = -INFINITY, inv = l_row == 0.f ? 0.f : 1.0f / l_row;
+            float M = -INFINITY;
+            // a row that sees no key is zeros; one whose keys all score -inf has l = 0 and comes out as 0 / 0
+            float inv = qpos < 0 ? 0.f : 1.0f / l_row;
             auto ml_of = [&](uint32_t i) {
                 return __ldcg(reinterpret_cast<const float2*>(
                     &p.part_ml[(static_cast<size_t>(piece_slot(u.c_first, i)) * BM + r) * 2]));
@@ -888,7 +890,7 @@ __global__ void __launch_bounds__(TCfg<HD, ACT == YATTN_ACT_F32, PAIR>::THREADS,
                         const float2 ml = ml_of(i);
                         l += (ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - M)) * ml.y;
                     }
-                    inv = l == 0.f ? 0.f : 1.0f / l;
+                    inv = qpos < 0 ? 0.f : 1.0f / l;
                 }
             }
             if (write) {
@@ -912,8 +914,8 @@ __global__ void __launch_bounds__(TCfg<HD, ACT == YATTN_ACT_F32, PAIR>::THREADS,
                                 o0[k] = __ldcg(s0 + k * BM);
                                 o1[k] = __ldcg(s1 + k * BM);
                             }
-                            const float w0 = m0 == -INFINITY ? 0.f : ex2_approx(m0 - M) * inv;
-                            const float w1 = m1 == -INFINITY || i1 == i ? 0.f : ex2_approx(m1 - M) * inv;
+                            const float w0 = (m0 == -INFINITY ? 0.f : ex2_approx(m0 - M)) * inv;
+                            const float w1 = i1 == i ? 0.f : (m1 == -INFINITY ? 0.f : ex2_approx(m1 - M)) * inv;
 #pragma unroll
                             for (int k = 0; k < 8; ++k) {
                                 x[4 * k] += w0 * o0[k].x + w1 * o1[k].x;
