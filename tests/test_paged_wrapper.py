@@ -18,3 +18,45 @@ def test_workspaces_are_dropped_after_any_status(monkeypatch, code, kept, clear)
     monkeypatch.setattr(attn, "_paged_ws", ws)
     assert attn.device_status(clear=clear) == code
     assert bool(ws) == kept
+
+
+def test_strides_past_32_bits_are_refused():
+    """The library takes strides as 32-bit numbers: one that does not fit would read other rows."""
+    from yllm_b200 import attn
+    meta = lambda stride, dt: torch.empty_strided((2, 256), (stride, 1), dtype=dt, device="meta")
+    for stride, fits in ((256, True), (2 ** 32 - 8, True), (2 ** 32, False), (2 ** 32 + 256, False)):
+        t, tables = meta(stride, torch.float16), meta(stride, torch.int32)
+        dev = t.get_device()
+        if fits:
+            assert attn._token_stride(t, "q", 2, 256, torch.float16, dev) == stride
+            assert attn._table_shape(tables, dev, 2) == (256, stride)
+            continue
+        with pytest.raises(ValueError, match="q must be"):
+            attn._token_stride(t, "q", 2, 256, torch.float16, dev)
+        with pytest.raises(ValueError, match="tables must be"):
+            attn._table_shape(tables, dev, 2)
+    one = torch.empty_strided((1, 256), (2 ** 40, 1), dtype=torch.float16, device="meta")   # a single row has no stride
+    assert attn._token_stride(one, "q", 1, 256, torch.float16, one.get_device()) == 256
+
+
+@pytest.mark.parametrize("max_new,given", [(-1, None), (0, 0), (3, 3), (2 ** 32, 2 ** 32 - 1), (2 ** 32 + 1, 2 ** 32 - 1)])
+def test_max_new_reaches_the_library_as_it_is_meant(monkeypatch, max_new, given):
+    """An upper bound that does not fit 32 bits stays an upper bound; a negative one is refused."""
+    from yllm_b200 import attn
+    seen = []
+    monkeypatch.setattr(attn, "_act_of", lambda q: (1, q.dtype, q.get_device(), q.shape[0]))
+    monkeypatch.setattr(attn, "_call_on", lambda name, dev, stream, *args: seen.append((name, args)))
+    e = lambda *s, dt=torch.float16: torch.zeros(*s, dtype=dt)
+    i32 = torch.int32
+    args = (e(4, 256), e(4, 256), e(2, 16, 128), e(2, 16, 128), e(1, 3, dt=i32), e(2, dt=i32), e(1, dt=i32), max_new, 4, 2, 64)
+    if given is None:
+        with pytest.raises(ValueError, match="max_new"):
+            attn.attn_paged(*args, workspace=e(16))
+        return
+    attn.attn_paged(*args, workspace=e(16))
+    (name, passed), = seen
+    names = ("out out_stride q q_stride gate gate_stride act kpool vpool n_pages page_size tables max_pages table_stride "
+             "cu_new kv_len n_seqs n_tokens max_new n_heads n_kv_heads head_dim kv_dim workspace workspace_bytes").split()
+    got = dict(zip(names, passed))
+    assert name == "yattn_attn_paged" and len(passed) == len(names)
+    assert (got["max_new"], got["n_tokens"], got["n_heads"], got["q_stride"]) == (given, 4, 4, 256)

@@ -406,6 +406,7 @@ def gemv_f16(y: torch.Tensor, w: torch.Tensor, x: torch.Tensor, out: int, in_: i
 
 _ACT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # YATTN_ACT_*
 _F16_BITS = (torch.float16, torch.uint16, torch.int16)
+_U32 = 0xFFFFFFFF   # a larger number would reach the library without its upper bits
 
 
 _tls = threading.local()   # err: this thread's message buffer
@@ -450,7 +451,7 @@ def _table_shape(tables: torch.Tensor, dev: int, n: int) -> tuple:
         stride, one = tables.stride()
         if rows == 1 and width > 0:
             stride = width
-        if rows == n and width > 0 and (one == 1 or width == 1) and stride >= width:
+        if rows == n and width > 0 and (one == 1 or width == 1) and width <= stride <= _U32:
             return width, stride
     raise ValueError(f"tables must be an int32 [{n} requests, pages] tensor on cuda:{dev} with contiguous rows")
 
@@ -474,9 +475,9 @@ def _token_stride(t: torch.Tensor, name: str, rows: int, cols: int, dtype: torch
         stride, one = t.stride()
         if rows == 1:
             stride = cols
-        if n == rows and m == cols and one == 1 and (stride >= cols or n == 0):
+        if n == rows and m == cols and one == 1 and (cols <= stride <= _U32 or n == 0):
             return stride
-    raise ValueError(f"{name} must be [{rows}, {cols}] {dtype} on cuda:{dev}, heads contiguous")
+    raise ValueError(f"{name} must be [{rows}, {cols}] {dtype} on cuda:{dev}, heads contiguous, tokens less than 2^32 elements apart")
 
 
 def _act_of(q: torch.Tensor) -> tuple:
@@ -574,6 +575,8 @@ def attn_paged(out: torch.Tensor, q: torch.Tensor, kpool: torch.Tensor, vpool: t
     width, stride = _table_shape(tables, dev, n)
     if cu_new.numel() != n + 1:
         raise ValueError("cu_new must have one entry more than kv_len")
+    if max_new < 0:
+        raise ValueError(f"max_new {max_new} is negative")
     if workspace is None:
         workspace = _paged_workspace(head_dim, dev, stream)
     elif workspace.get_device() != dev or not workspace.is_contiguous():
@@ -582,7 +585,7 @@ def attn_paged(out: torch.Tensor, q: torch.Tensor, kpool: torch.Tensor, vpool: t
              q.data_ptr(), _token_stride(q, "q", rows, cols, dtype, dev), None if gate is None else gate.data_ptr(),
              0 if gate is None else _token_stride(gate, "gate", rows, cols, dtype, dev), act, kpool.data_ptr(),
              vpool.data_ptr(), pages, page_size, tables.data_ptr(), width, stride, cu_new.data_ptr(),
-             kv_len.data_ptr(), n, rows, max_new, n_heads, n_kv_heads, head_dim, kv_dim, workspace.data_ptr(),
+             kv_len.data_ptr(), n, rows, min(max_new, _U32), n_heads, n_kv_heads, head_dim, kv_dim, workspace.data_ptr(),
              workspace.nbytes)
 
 
