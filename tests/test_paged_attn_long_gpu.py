@@ -76,3 +76,26 @@ def test_long_pieces_of_random_scores(dev, act, hd, H, KV, L, n, large):  # noqa
         c.run()
         assert torch.equal(c.out, first)
     assert bool((c.out[c.total:] == 3.0).all())
+
+
+def test_own_workspace_on_another_stream(dev):  # noqa: F811
+    """paged_workspace() zeroes its counters behind work of the current stream; a call on another stream does not wait
+    for that stream, and may come at once."""
+    from yllm_b200 import attn
+    c = Case(dev, 32, 8, 128, 64, [30000], [1], seed=50)
+    s = torch.cuda.Stream()
+    c.run(stream=s)
+    torch.cuda.synchronize()
+    good = c.out.clone()
+    c.out.fill_(3.0)
+    junk = torch.full((attn.paged_workspace(128).numel(),), 255, dtype=torch.uint8, device=dev)
+    torch.cuda.synchronize()
+    at = junk.data_ptr()
+    del junk
+    torch.cuda._sleep(200_000_000)                     # about 0.1 s on the current stream
+    ws = attn.paged_workspace(128)
+    assert ws.data_ptr() == at                         # (the memory that is not zero)
+    c.run(workspace=ws, stream=s)
+    s.synchronize()
+    torch.cuda.synchronize()
+    assert attn.device_status() == 0 and torch.equal(c.out, good)

@@ -60,3 +60,17 @@ def test_max_new_reaches_the_library_as_it_is_meant(monkeypatch, max_new, given)
     got = dict(zip(names, passed))
     assert name == "yattn_attn_paged" and len(passed) == len(names)
     assert (got["max_new"], got["n_tokens"], got["n_heads"], got["q_stride"]) == (given, 4, 4, 256)
+
+
+def test_workspace_is_made_on_the_device_that_is_named(monkeypatch):
+    """Device 0 is a device, not the default."""
+    from yllm_b200 import attn
+    made = []
+    monkeypatch.setattr(attn, "_new_workspace", lambda head_dim, dev: made.append((head_dim, dev)))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 5)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    for device in (0, "cuda:0", torch.device("cuda", 0), 3, None, "cuda"):
+        attn.paged_workspace(128, device)
+    assert made == [(128, d) for d in (0, 0, 0, 3, 5, 5)]
+    with pytest.raises(ValueError, match="CUDA"):
+        attn.paged_workspace(128, "cpu")

@@ -536,10 +536,24 @@ def rope_store_kv_paged(q_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
 _paged_ws: dict = {}   # (device, stream, head_dim) -> workspace of attn_paged's eager calls on that stream
 
 
+def _new_workspace(head_dim: int, dev: int) -> torch.Tensor:
+    """A workspace whose counters are zeroed in the order of the current stream of dev."""
+    with torch.cuda.device(dev):
+        ws = torch.empty(lib.yattn_attn_paged_workspace_bytes(head_dim), dtype=torch.uint8, device=torch.device("cuda", dev))
+        ws[:4096].zero_()
+    return ws
+
+
 def paged_workspace(head_dim: int, device=None) -> torch.Tensor:
-    """A workspace for attn_paged (its counters zeroed), for callers that keep their own (one per stream or graph in flight)."""
-    ws = torch.empty(lib.yattn_attn_paged_workspace_bytes(head_dim), dtype=torch.uint8, device=device or "cuda")
-    ws[:4096].zero_()
+    """A workspace for attn_paged (its counters zeroed), for callers that keep their own (one per stream or graph in
+    flight).  Made outside a capture, it is ready for any stream when the call returns."""
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError(f"paged_workspace: {device} is not a CUDA device")
+    dev = torch.cuda.current_device() if device.index is None else device.index
+    ws = _new_workspace(head_dim, dev)
+    if not torch.cuda.is_current_stream_capturing():
+        torch.cuda.current_stream(dev).synchronize()
     return ws
 
 
@@ -553,11 +567,11 @@ def _paged_workspace(head_dim: int, dev: int, stream) -> torch.Tensor:
         with torch.cuda.device(dev):
             return _paged_workspace(head_dim, dev, None)
     if _capturing():
-        return paged_workspace(head_dim, torch.device("cuda", dev))
+        return _new_workspace(head_dim, dev)
     key = (dev, _raw_stream(dev), head_dim)
     ws = _paged_ws.get(key)
     if ws is None:
-        ws = _paged_ws[key] = paged_workspace(head_dim, torch.device("cuda", dev))
+        ws = _paged_ws[key] = _new_workspace(head_dim, dev)
     return ws
 
 
