@@ -74,3 +74,33 @@ def test_workspace_is_made_on_the_device_that_is_named(monkeypatch):
     assert made == [(128, d) for d in (0, 0, 0, 3, 5, 5)]
     with pytest.raises(ValueError, match="CUDA"):
         attn.paged_workspace(128, "cpu")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_norm_weights_are_held_and_checked(monkeypatch, dtype):
+    """The struct has bare pointers: the weights live as long as it does, and each call checks their size."""
+    import gc
+    import weakref
+
+    from yllm_b200 import attn
+    with pytest.raises(ValueError, match="q_w must be a CUDA"):
+        attn.qk_norm(torch.ones(128, dtype=dtype), torch.ones(128, dtype=dtype), 1e-6)
+    monkeypatch.setattr(attn, "_need", lambda t, dt, name: None)
+    q_w, k_w = torch.ones(128, dtype=dtype), torch.ones(128, dtype=dtype)
+    alive = weakref.ref(q_w)
+    norm = attn.qk_norm(q_w, k_w, 1e-6)
+    assert norm.q_w == q_w.data_ptr() and norm.k_w == k_w.data_ptr() and norm.w_f16 == (dtype == torch.float16)
+    del q_w
+    gc.collect()
+    assert alive() is not None
+    assert attn._norm_arg(None, 64) is None
+    attn._norm_arg(norm, 128)
+    attn._norm_arg(norm, 128, -1)
+    with pytest.raises(ValueError, match="128 values for head_dim 256"):
+        attn._norm_arg(norm, 256)
+    with pytest.raises(ValueError, match="cuda:0"):
+        attn._norm_arg(norm, 128, 0)
+    attn._norm_arg(attn.YattnQkNorm(1, 2, 0, 1e-6), 256)      # a struct of the caller's own has pointers only
+    norm = attn.qk_norm(torch.ones(64, dtype=dtype), torch.ones(32, dtype=dtype), 1e-6)
+    with pytest.raises(ValueError, match="32 values"):
+        attn._norm_arg(norm, 64)

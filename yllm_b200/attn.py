@@ -253,14 +253,23 @@ def qk_norm(q_w: torch.Tensor, k_w: torch.Tensor, eps: float):
     f16 = q_w.dtype in (torch.int16, torch.uint16, torch.float16)
     if f16 != (k_w.dtype in (torch.int16, torch.uint16, torch.float16)):
         raise ValueError("q and k norm weights must have the same dtype")
-    if not f16:
-        _need(q_w, torch.float32, "q_w")
-        _need(k_w, torch.float32, "k_w")
-    return YattnQkNorm(q_w.data_ptr(), k_w.data_ptr(), 1 if f16 else 0, float(eps))
+    for name, w in (("q_w", q_w), ("k_w", k_w)):
+        _need(w, w.dtype if f16 else torch.float32, name)
+    norm = YattnQkNorm(q_w.data_ptr(), k_w.data_ptr(), 1 if f16 else 0, float(eps))
+    norm.weights = (q_w, k_w)   # lives as long as the pointers to it
+    return norm
 
 
-def _norm_arg(norm):
-    return None if norm is None else C.byref(norm)
+def _norm_arg(norm, head_dim: int, dev: Optional[int] = None):
+    """The call's pointer to norm; weights that qk_norm holds must be head_dim values (on device dev, where given)."""
+    if norm is None:
+        return None
+    for w in getattr(norm, "weights", ()):
+        if w.numel() != head_dim:
+            raise ValueError(f"QK-norm weights have {w.numel()} values for head_dim {head_dim}")
+        if dev is not None and w.get_device() != dev:
+            raise ValueError(f"QK-norm weights must be on cuda:{dev}")
+    return C.byref(norm)
 
 
 def rope_store_kv(items: torch.Tensor, n_items: int, n_heads: int, n_kv_heads: int, head_dim: int, kv_dim: int,
@@ -269,7 +278,7 @@ def rope_store_kv(items: torch.Tensor, n_items: int, n_heads: int, n_kv_heads: i
     (engine.c:1052-1072 / cuda_fwd.c:136-147 for every item, one launch).  norm (qk_norm(...)) applies the
     per-head QK-norm first."""
     call("yattn_rope_store_kv", items.data_ptr(), n_items, n_heads, n_kv_heads, head_dim, kv_dim, rope_kind,
-         n_rope_dims, theta, _norm_arg(norm), _stream(stream))
+         n_rope_dims, theta, _norm_arg(norm, head_dim), _stream(stream))
 
 
 def rope_store_kv_batch(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kcache: torch.Tensor,
@@ -282,7 +291,7 @@ def rope_store_kv_batch(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kcach
         _need(t, torch.float32, name)
     call("yattn_rope_store_kv_batch", q.data_ptr(), k.data_ptr(), v.data_ptr(), kcache.data_ptr(), vcache.data_ptr(),
          pos_start, B, q_stride or n_heads * head_dim, n_heads, n_kv_heads, head_dim, kv_dim, rope_kind, n_rope_dims,
-         theta, _norm_arg(norm), _stream(stream))
+         theta, _norm_arg(norm, head_dim), _stream(stream))
 
 
 def decode_partial(ml: torch.Tensor, o: torch.Tensor, q: torch.Tensor, kcache: torch.Tensor, vcache: torch.Tensor,
@@ -530,7 +539,7 @@ def rope_store_kv_paged(q_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
              _token_stride(k, "k", rows, kv_cols, dtype, dev), v.data_ptr(),
              _token_stride(v, "v", rows, kv_cols, dtype, dev), act, kpool.data_ptr(), vpool.data_ptr(),
              pages * page_size, slots.data_ptr(), positions.data_ptr(), rows, n_heads, n_kv_heads, head_dim, kv_dim,
-             rope_kind, n_rope_dims, theta, _norm_arg(norm))
+             rope_kind, n_rope_dims, theta, _norm_arg(norm, head_dim, dev))
 
 
 _paged_ws: dict = {}   # (device, stream, head_dim) -> workspace of attn_paged's eager calls on that stream
