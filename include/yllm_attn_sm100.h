@@ -535,7 +535,8 @@ enum { YATTN_ACT_F32 = 0, YATTN_ACT_F16 = 1, YATTN_ACT_BF16 = 2 };   /* activati
  * after a 602 from this call tables and ring have to be set up anew.
  * The inputs kv_len, new_len and state stay as they are and must not overlap
  * the outputs: feed kv_len_out and state_out to the next step (two sets of
- * buffers in turn).  state_out is 16-byte aligned.  1 to 16384 requests. */
+ * buffers in turn).  state_out is 16-byte aligned.  1 to 16384 requests
+ * (yattn_attn_paged takes up to 65535). */
 int yattn_page_step(int32_t* kv_len_out, int32_t* cu_new, int32_t* slots, int32_t* positions,
                     uint32_t max_tokens, int32_t* state_out, int32_t* tables, uint32_t max_pages,
                     uint32_t table_stride, int32_t* ring, uint32_t n_pages, const int32_t* state,
@@ -574,7 +575,8 @@ int yattn_rope_store_kv_paged(void* q_out, uint32_t q_out_stride, const void* q,
  * (or NULL): out is multiplied by sigmoid(gate), as yattn_attn_prefill.
  * q, gate and out hold activations of type `act`, tokens *_stride elements
  * apart.  Rows from cu_new[n_seqs] on are not written; n_tokens is q's row
- * count.  max_new is an upper bound of the requests' new tokens (host): up to 8
+ * count.  max_new is an upper bound of the requests' new tokens (host; 0: nothing
+ * runs, nothing is checked on the device): up to 8
  * query rows per kv head (max_new * n_heads/n_kv_heads) run the decode form,
  * more run 128-row tiles on tcgen05; an fp32 batch of mostly such small requests
  * (n_seqs * n_kv_heads >= SMs, 4 n_tokens <= n_seqs * max_new) runs both, a launch
@@ -582,13 +584,16 @@ int yattn_rope_store_kv_paged(void* q_out, uint32_t q_out_stride, const void* q,
  * nothing here depends on them at capture time.
  * fp32 activations keep about 22 bits of q and of the softmax weights (fp16 hi
  * + lo planes); 16-bit activations run one plane of each in the tiles form
- * (bf16 q to 2^-19 or better of its row's largest).
+ * (bf16 q to 2^-19 or better of its row's largest, softmax weights to fp16's half
+ * step) and two in the decode form, so the same token may differ in its last bits
+ * between a decode step and a step with chunks.
  * A block table entry outside the pool reads as zero rows (device status 602);
  * a request whose offsets or lengths contradict the arguments, or which has
  * more than max_new tokens, is skipped, its rows of out not written (603).
  * Cache rows behind kv_len may hold anything.  A K or V row before it that is
  * not finite reaches every token that sees it, and such a V row may also reach
- * earlier tokens of its own chunk (0 * inf in a shared product).
+ * earlier tokens of its own chunk (0 * inf in a shared product).  A token all of
+ * whose keys score -inf is NaN (0 / 0).
  * head_dim 64/128/256, n_heads a multiple of n_kv_heads; out overlaps nothing.
  * workspace: yattn_attn_paged_workspace_bytes, its first 4096 bytes zeroed once; a
  * call leaves them zero.  Calls that may overlap (other streams, graphs) need

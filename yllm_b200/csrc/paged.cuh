@@ -41,7 +41,8 @@ struct PagedParams {
 };
 
 constexpr uint32_t kPagedCounters = 1024;        // most CTAs of a launch
-constexpr int kPagedMaxPieces = 5 * 32;          // a cut unit has at most one piece per CTA
+constexpr int kPagedMaxPieces = 5 * 32;          // decode form: most CTAs, each of which holds a piece of a unit at most
+                                                 // (the tiles' merge has no such bound; they run up to two CTAs per SM)
 
 // Activations of the call's type, as fp32.
 __device__ __forceinline__ float2 ld_act2(const void* p, size_t i, int act) {

@@ -44,9 +44,6 @@ template <int HD> struct RowsCfg {
     static_assert(NCW * 8 * HD * 4 <= STAGE, "the warps' o fit the unit's last stage");
 };
 
-// The two elements of a query row at element offset i, ACT a YATTN_ACT_*.
-template <int ACT> __device__ __forceinline__ float2 q_pair(const void* q, size_t i) { return ld_act2(q, i, ACT); }
-
 template <int HD, int HC>
 __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
     k_paged_rows(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -203,9 +200,9 @@ __global__ void __launch_bounds__(RowsCfg<HD>::THREADS, 1)
                     xb[kk] = hv ? pair(qa + kk * 16 + 8) : make_float2(0.f, 0.f);
                 }
             };
-            if (p.act == YATTN_ACT_F32) load([&](size_t i) { return q_pair<YATTN_ACT_F32>(p.q, i); });
-            else if (p.act == YATTN_ACT_F16) load([&](size_t i) { return q_pair<YATTN_ACT_F16>(p.q, i); });
-            else load([&](size_t i) { return q_pair<YATTN_ACT_BF16>(p.q, i); });
+            if (p.act == YATTN_ACT_F32) load([&](size_t i) { return ld_act2(p.q, i, YATTN_ACT_F32); });
+            else if (p.act == YATTN_ACT_F16) load([&](size_t i) { return ld_act2(p.q, i, YATTN_ACT_F16); });
+            else load([&](size_t i) { return ld_act2(p.q, i, YATTN_ACT_BF16); });
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk)
                 mx = fmaxf(mx, fmaxf(fmaxf(fabsf(xa[kk].x), fabsf(xa[kk].y)), fmaxf(fabsf(xb[kk].x), fabsf(xb[kk].y))));

@@ -7,7 +7,8 @@
 // The pairs are those of the contiguous store (rope.cu).  The angle differs on purpose: there it is one
 // fp32 multiply, as in the reference's engine, which at position 100,000 is off by up to 2^-8 rad (half
 // an ulp of the angle); here it is a product in 64 bits, reduced to a half turn before it is rounded, so
-// every angle is good to 1 ulp of its sine and cosine however far the position.
+// sine and cosine are off by 2^-22 or less, absolute, however far the position: 2^-24 or so for the angle's
+// rounding and 2 ulp for sincospif, which is 2^-22 of the pair's norm.
 //
 // A thread holds two VEC-element chunks of one head, VEC * size = 16 bytes, placed so that both elements
 // of each of its pairs are its own (half-split pairs: chunk c and chunk c + n/2; neighbour pairs and
