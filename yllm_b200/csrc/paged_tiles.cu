@@ -10,8 +10,8 @@
 // is fetched, below), else scaled as fp32 is.  P's half step 2^-11 is far below the output's own rounding at bf16
 // and equal to it at fp16, where it adds to it: fp16 outputs are off by 1.15 (20 keys) to 1.45 (30,000 keys) times
 // what fp32 arithmetic rounded once is.  P carries a factor 2^7 (it cancels in O / l): kPUp.
-// The tensor core truncates where it adds to an accumulator, always towards zero, so PREC issues Q_lo K before Q_hi K, sums at most 256 keys
-// of P V in one accumulator and adds those sums in fp32 (the fold below).  Over 8700 keys the result was off
+// The tensor core truncates where it adds to an accumulator, always towards zero, so PREC issues Q_lo K before
+// Q_hi K, sums at most 256 keys of P V in one accumulator and adds those sums in fp32 (the fold below).  Over 8700 keys the result was off
 // by 1.1e-5 without that, 2.6e-6 with sums of 1024 keys, 0.9e-6 with 256 (elementary fp32 operations: 1.3e-6),
 // for 1 % of the time at head_dim 128 and 15 % at 256, where the fold goes through global memory.  16-bit
 // activations sum 8192 keys, through global memory too: the drift stays under 2^-14 of the result, far below its
